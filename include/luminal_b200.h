@@ -584,6 +584,74 @@ int32_t lmb200_decode_attention_noalloc(lmb200_ctx ctx, int32_t dtype, const voi
                                         int32_t batch, int32_t n_kv_heads, int32_t group,
                                         int32_t head_dim, int32_t T);
 
+/* ---------------------------------------------------------------------------------------------
+ * A paged key / value cache held in 4 bits, its block tables on the device, and the verification of drafted tokens.  For callers that
+ * serve many sequences with their own model code: every array is the caller's device memory, the calls are asynchronous on the context's
+ * stream, allocate nothing and may be recorded (lmb200_capture_begin).  Sizes that only the device knows (how many tokens a step has, how long
+ * a sequence is) are read there, so a recorded step serves every later one.  The reference has no counterpart: its only cache is one
+ * dense array per layer and sequence (src/Whisper.jl:519-541) and its loop takes one greedy token at a time (src/Decoding.jl:91-130).
+ *
+ * A step of a serving loop:  lmb200_kv_reserve (lengths + new tokens -> pages, slots), per layer lmb200_kv4_append and lmb200_kv4_attention,
+ * lmb200_verify_drafts on the logits, lmb200_kv_shrink by its `drop`.
+ *
+ * The cache of one layer is n_pages pages of page_size tokens (16, 32, 64, 128 or 256); head_dim is a multiple of 32 up to 256.  Values are held per token,
+ * kv head and 32 neighbouring features as m + n s: m the half-precision number nearest the smallest of the 32, s the one nearest float32((largest - smallest) / 15),
+ * n = rint(float32((x - m) / s)) within 0..15 (0 where s is 0).  A group that has a NaN, or whose m or s is not finite, reads back as NaN.
+ * lmb200_kv4_page_bytes bytes a page, [kv head][token / 16][20 head_dim bytes]; inside a block of 16 tokens, with g = d / 32 and t16 = token % 16:
+ *   bytes 0 .. 8 D - 1       keys: 4-byte words [g][t16 % 8][d % 8 / 2][d / 16 % 2], byte 2 (d % 2) + t16 / 8 of the word, low half if d % 16 < 8, else high half
+ *   bytes 8 D .. 16 D - 1    values: 4-byte words [g][d % 8][t16 % 8 / 2][d / 16 % 2], byte 2 (t16 % 2) + t16 / 8 of the word, low half if d % 16 < 8, else high half
+ *   then float16, D each     key s and key m [g][t16 % 8][t16 / 8]; value s and value m [g][t16 % 8 / 2][t16 / 8][t16 % 2]
+ * A slot is page * page_size + place in the page.  The places of a cache that no call has written are the caller's (zeros read back as 0).
+ *
+ * A slot or a table entry outside the cache, or row offsets outside the rows, touch no memory: they are left out and the next synchronising call
+ * returns LMB200_EINVAL.
+ * ------------------------------------------------------------------------------------------ */
+int32_t lmb200_kv4_page_bytes(int32_t page_size, int32_t n_kv_heads, int32_t head_dim, int64_t* bytes);
+/* Room for add[b] >= 0 more tokens of every sequence b < n_seq (at most 8192).  A sequence of `lens` tokens holds the first ceil(lens / page_size) pages of its row of
+ * table [n_seq, max_pages]; free_list [n_pages] holds n_free[0] free pages, the next one to take last.  Writes the new pages into the table, lens_out [n_seq] = lens + add,
+ * n_free_out [1], cu_rows [n_seq + 1] (the new tokens are packed in order of the sequences; sequence b has the rows cu_rows[b] .. cu_rows[b + 1] - 1) and slots [rows], -1
+ * behind the last token.  lens_out may be lens and n_free_out n_free.  All or nothing: if the tokens do not fit, nothing is taken, cu_rows is 0, the
+ * slots are -1, and status [1] says why as a sum of 1 (too few free pages), 2 (more tokens than rows), 4 (a sequence longer than its row of the table),
+ * 8 (a negative number, or n_free outside the list); else status is 0.  The reference has no counterpart (src/Whisper.jl:519-541: one array per sequence). */
+int32_t lmb200_kv_reserve(lmb200_ctx ctx, int32_t n_seq, int32_t page_size, int32_t max_pages, int32_t n_pages, int32_t rows, const int32_t* lens, const int32_t* add,
+                          int32_t* table, const int32_t* free_list, const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out, int32_t* cu_rows, int32_t* slots,
+                          int32_t* status);
+/* The last drop[b] tokens of every sequence leave the cache (drop <= 0: none; drop >= lens[b]: all, the sequence has ended): lens_out = max(0, lens - drop), and the pages
+ * that no token needs any more go back to the free list in the reverse of the order in which kv_reserve takes them.  lens_out may be lens and n_free_out
+ * n_free.  If lengths, tables and list do not fit together nothing is given back and the next synchronising call returns LMB200_EINVAL. */
+int32_t lmb200_kv_shrink(lmb200_ctx ctx, int32_t n_seq, int32_t page_size, int32_t max_pages, int32_t n_pages, const int32_t* lens, const int32_t* drop, const int32_t* table,
+                         int32_t* free_list, const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out);
+/* Stores k and v [rows, n_kv_heads, head_dim] (dtype F32 or BF16; rows k_stride / v_stride elements apart, each on a 16-byte boundary) at slots [rows]; a row whose slot is
+ * negative is skipped.  No two rows may have the same slot. */
+int32_t lmb200_kv4_append(lmb200_ctx ctx, int32_t dtype, const void* k, const void* v, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads,
+                          int32_t head_dim, const int32_t* slots, void* pages, int32_t n_pages, int32_t page_size);
+/* The values that the cache holds at slots [rows], into k_out and v_out; rows whose slot is negative are left as they are. */
+int32_t lmb200_kv4_read(lmb200_ctx ctx, int32_t dtype, void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads, int32_t head_dim,
+                        const int32_t* slots, const void* pages, int32_t n_pages, int32_t page_size);
+/* out = softmax(scale q K^T) V over the cache, causal: the rows of sequence b (cu_rows as above) are its last tokens, each sees itself and every token before it, or
+ * the last `window` of them (0: all).  `lens` counts the rows' own tokens, so they are appended first.  q and out: [rows, n_kv_heads * group, head_dim] in dtype, the query
+ * heads of a kv head side by side, rows q_stride / out_stride elements apart, each on a 16-byte boundary.  Rows behind cu_rows[n_seq] are left as they are; a row that sees
+ * no key is 0.  Scores, softmax and sums in float32.  workspace: lmb200_kv4_attention_workspace bytes, zero before its first use (every call leaves it
+ * usable for the next); calls that may run at the same time need one each. */
+int32_t lmb200_kv4_attention_workspace(lmb200_ctx ctx, int32_t head_dim, int64_t* bytes);
+int32_t lmb200_kv4_attention(lmb200_ctx ctx, int32_t dtype, const void* q, int64_t q_stride, void* out, int64_t out_stride, int32_t rows, int32_t n_seq, const int32_t* cu_rows,
+                             const int32_t* lens, const int32_t* table, int32_t max_pages, const void* pages, int32_t n_pages, int32_t page_size, int32_t n_kv_heads,
+                             int32_t group, int32_t head_dim, float scale, int32_t window, void* workspace, int64_t workspace_bytes);
+/* Speculative decoding: row r of `target` [rows, vocab] holds the target model's logits behind tokens[r], the rows of sequence b being cu_rows[b] .. cu_rows[b + 1] - 1; the
+ * tokens behind a sequence's first row are drafts, and each is judged by the row before it.  With p = softmax(target / T), T = temperature[b], and q = softmax(draft / T)
+ * (draft [rows, vocab]: the draft model's logits in the same rows; NULL: the drafts were certain) a draft t is taken where accept_u[r] q(t) < p(t).  The first row r that takes no draft,
+ * or the sequence's last row, gives one new token: the smallest j whose sum of max(p - q, 0) (the last row: of p) over 0 .. j exceeds sample_u[b] of the whole.  The
+ * tokens that come out follow the target's distribution.  temperature NULL or T not above 0: a draft is taken where it is the row's largest logit (the first of equals), and
+ * that is the new token.  Random numbers are uniform in [0, 1), accept_u [rows], sample_u [n_seq].  A NaN counts as -infinity, +infinity as the largest float; a row of
+ * -infinities takes nothing and gives -1.
+ * tokens_out[rows]: per sequence the taken drafts, the new token, then -1 up to its last row; n_out[b]: how many tokens those are (0 for a sequence without rows); drop[b]: how many drafts
+ * were refused, for lmb200_kv_shrink.  Rows behind cu_rows[n_seq] are left as they are.  target and draft in dtype (F32 or BF16), rows apart by the strides.  workspace:
+ * lmb200_verify_drafts_workspace(rows) bytes, in any state.  Stands beside lmb200_argmax; replaces the choice of one token (src/Decoding.jl:119-124). */
+int32_t lmb200_verify_drafts_workspace(int32_t rows, int64_t* bytes);
+int32_t lmb200_verify_drafts(lmb200_ctx ctx, int32_t dtype, const void* target, int64_t target_stride, const void* draft, int64_t draft_stride, int32_t vocab, int32_t rows,
+                             int32_t n_seq, const int32_t* cu_rows, const int32_t* tokens, const float* temperature, const float* accept_u, const float* sample_u,
+                             int32_t* tokens_out, int32_t* n_out, int32_t* drop, void* workspace, int64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -134,6 +134,15 @@ SIGNATURES = {
     "lmb200_compile_node_list": [_u64, _vp, _i32, _vp, _i32, _i32, _i32, _i32, C.POINTER(_u64), C.POINTER(_u64), _vp],
     "lmb200_decode_attention_splitkv": [_u64, _i32, _vp, _vp, _i32],
     "lmb200_session_kv_layer": [_u64, _i32, C.POINTER(_vp), _pi64, _pi64],
+    "lmb200_kv4_page_bytes": [_i32, _i32, _i32, _pi64],
+    "lmb200_kv_reserve": [_u64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "lmb200_kv_shrink": [_u64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "lmb200_kv4_append": [_u64, _i32, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _i32],
+    "lmb200_kv4_read": [_u64, _i32, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _i32],
+    "lmb200_kv4_attention_workspace": [_u64, _i32, _pi64],
+    "lmb200_kv4_attention": [_u64, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i64],
+    "lmb200_verify_drafts_workspace": [_i32, _pi64],
+    "lmb200_verify_drafts": [_u64, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64],
     "lmb200_decode_attention_noalloc": [_u64, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32],
 }
 

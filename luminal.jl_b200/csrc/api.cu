@@ -11,6 +11,7 @@
 #include "common.cuh"
 #include "recorded.cuh"
 #include "gemv.cuh"
+#include "kv4.cuh"
 #include "model.cuh"
 #include "pdl.cuh"
 
@@ -18,6 +19,7 @@ namespace lmb {
 
 int32_t flash_tc_configure();
 int32_t flash_tc_f32_configure();
+int32_t paged_configure();
 
 static thread_local char g_err[1024] = "";
 
@@ -56,6 +58,10 @@ int32_t check_device_error(Ctx* ctx) {
   const int code = ctx->dev_err ? *reinterpret_cast<volatile int*>(ctx->dev_err) : 0;
   if (code != 0) {
     *ctx->dev_err = 0;
+    if (code == kv4::kErrPage)
+      return fail(LMB200_EINVAL, "a slot, a block table or a row offset names a place outside its cache or its rows: what it named was left out of the results");
+    if (code == kv4::kErrFree)
+      return fail(LMB200_EINVAL, "kv_shrink: lengths, block tables and free list do not fit together; nothing was given back");
     if (ctx->nccl_comm && ctx->tp_size > 1) ctx->comm_broken = true;
     if (code == 2)
       return fail(LMB200_ETIMEOUT, "a peer rank's signal was invalid (that rank had a wait run out, or the ranks' step counters "
@@ -330,6 +336,7 @@ extern "C" int32_t lmb200_init(int32_t device, lmb200_ctx* out) {
   if (rc == LMB200_OK) rc = step_kernels_configure();
   if (rc == LMB200_OK) rc = prefill_configure();
   if (rc == LMB200_OK) rc = layered_configure();
+  if (rc == LMB200_OK) rc = paged_configure();
   if (rc != LMB200_OK) { cudaFree(c->dev_broken); cudaFreeHost(c->dev_err); cudaStreamDestroy(c->own_stream); delete c; return rc; }
   *out = reinterpret_cast<lmb200_ctx>(c);
   return LMB200_OK;

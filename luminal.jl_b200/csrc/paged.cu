@@ -1,0 +1,415 @@
+// Block tables on the GPU (lmb200_kv_reserve, lmb200_kv_shrink) and the 4-bit cache's store and load (lmb200_kv4_append, lmb200_kv4_read).
+#include <limits.h>
+
+#include "kv4.cuh"
+#include "pdl.cuh"
+
+namespace lmb {
+namespace {
+
+constexpr int kTableThreads = 1024;
+constexpr int kMaxSeqs = 8192;               // three words of shared memory each
+
+struct TableParams {
+  int n_seq, shift, max_pages, n_pages, rows;
+  const int *lens, *change, *n_free;
+  int *table, *free_list;                    // reserve writes the table, shrink the free list
+  int *lens_out, *n_free_out, *cu_rows, *slots, *status;
+  int* dev_err;
+};
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ int cluster_rank() { int r; asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
+__device__ __forceinline__ int cluster_size() { int r; asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r)); return r; }
+
+// Exclusive sums over the block of two counts per thread, and their totals.
+__device__ __forceinline__ void scan2(long long a, long long b, long long& ea, long long& eb, long long& ta, long long& tb) {
+  __shared__ long long sa[32], sb[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long ia = a, ib = b;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long ua = __shfl_up_sync(0xffffffffu, ia, off), ub = __shfl_up_sync(0xffffffffu, ib, off);
+    if (lane >= off) { ia += ua; ib += ub; }
+  }
+  if (lane == 31) { sa[warp] = ia; sb[warp] = ib; }
+  __syncthreads();
+  if (warp == 0) {
+    long long va = sa[lane], vb = sb[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long ua = __shfl_up_sync(0xffffffffu, va, off), ub = __shfl_up_sync(0xffffffffu, vb, off);
+      if (lane >= off) { va += ua; vb += ub; }
+    }
+    sa[lane] = va;
+    sb[lane] = vb;
+  }
+  __syncthreads();
+  ea = ia - a + (warp ? sa[warp - 1] : 0);
+  eb = ib - b + (warp ? sb[warp - 1] : 0);
+  ta = sa[31];
+  tb = sb[31];
+}
+
+// the last index in [lo, hi] with at[index] <= x (at ascending, at[lo] <= x)
+__device__ __forceinline__ int last_at_most(const int* at, int lo, int hi, int x) {
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (at[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// One cluster.  Every CTA reads all lengths and forms the same sums (a thread takes neighbouring sequences); behind the cluster's barrier, when
+// nobody reads them any more, the outputs, which may be the inputs' arrays, are written.  Rows and pages are dealt out to all warps in groups
+// of 32 neighbours, whose sequence is found by bisection.
+__global__ void __launch_bounds__(kTableThreads) reserve_kernel(const TableParams p) {
+  extern __shared__ int sm[];
+  int* len = sm;
+  int* row0 = len + p.n_seq;                 // first row of a sequence
+  int* page0 = row0 + p.n_seq;               // its first new page
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, per = (p.n_seq + kTableThreads - 1) / kTableThreads;
+  const int first = min(tid * per, p.n_seq), last = min(first + per, p.n_seq);
+  const int free_now = *p.n_free, size1 = (1 << p.shift) - 1;
+  long long rows = 0, pages = 0;
+  int bad = 0;
+  for (int b = first; b < last; ++b) {
+    const long long l = p.lens[b], a = p.change[b];
+    if (l < 0 || a < 0) { bad |= 8; continue; }
+    if (((l + a + size1) >> p.shift) > p.max_pages) bad |= 4;
+    rows += a;
+    pages += ((l + a + size1) >> p.shift) - ((l + size1) >> p.shift);
+  }
+  long long er, ep, tr, tp;
+  scan2(rows, pages, er, ep, tr, tp);
+  bad = __syncthreads_or(bad & 8 ? 1 : 0) * 8 | __syncthreads_or(bad & 4 ? 1 : 0) * 4;
+  if (tr > p.rows) bad |= 2;
+  if (free_now < 0 || free_now > p.n_pages) bad |= 8;
+  else if (tp > free_now) bad |= 1;
+  if (!bad)
+    for (int b = first; b < last; ++b) {
+      const long long l = p.lens[b], a = p.change[b];
+      len[b] = (int)l;
+      row0[b] = (int)er;
+      page0[b] = (int)ep;
+      er += a;
+      ep += ((l + a + size1) >> p.shift) - ((l + size1) >> p.shift);
+    }
+  __syncthreads();
+  const int n_rows = bad ? 0 : (int)tr, n_new = bad ? 0 : (int)tp;
+  const int lane = tid & 31, warps = kTableThreads / 32 * cluster_size(), warp = cluster_rank() * (kTableThreads / 32) + (tid >> 5);
+  // slots: the token's page is a new one, or the last that its sequence holds.  (`table` is read at places that this call does not write.)
+  for (int r0 = warp * 32; r0 < p.rows; r0 += warps * 32) {
+    const int r = r0 + lane;
+    int slot = -1;
+    if (r0 < n_rows) {
+      const int lo = last_at_most(row0, 0, p.n_seq - 1, r0);
+      const int hi = last_at_most(row0, lo, p.n_seq - 1, min(r0 + 31, n_rows - 1));
+      if (r < n_rows) {
+        const int b = lo == hi ? lo : last_at_most(row0, lo, hi, r);
+        const int pos = len[b] + (r - row0[b]);
+        const int j = (pos >> p.shift) - ((len[b] + size1) >> p.shift);
+        const int page = j >= 0 ? p.free_list[free_now - 1 - (page0[b] + j)] : p.table[(int64_t)b * p.max_pages + (pos >> p.shift)];
+        if ((unsigned)page < (unsigned)p.n_pages) slot = (page << p.shift) + (pos & size1);
+      }
+    }
+    if (r < p.rows) p.slots[r] = slot;
+  }
+  for (int k0 = warp * 32; k0 < n_new; k0 += warps * 32) {
+    const int k = k0 + lane;
+    if (k < n_new) {
+      const int b = last_at_most(page0, 0, p.n_seq - 1, k);
+      p.table[(int64_t)b * p.max_pages + ((len[b] + size1) >> p.shift) + (k - page0[b])] = p.free_list[free_now - 1 - k];
+    }
+  }
+  if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();   // lens and n_free are read by no one any more
+  if (cluster_rank() != 0) return;
+  for (int b = tid; b < p.n_seq; b += kTableThreads) {
+    const int up = b + 1 < p.n_seq ? row0[b + 1] : n_rows;
+    if (!bad) p.lens_out[b] = len[b] + up - row0[b];
+    else if (p.lens_out != p.lens) p.lens_out[b] = p.lens[b];
+    p.cu_rows[b + 1] = bad ? 0 : up;
+  }
+  if (tid == 0) {
+    p.cu_rows[0] = 0;
+    *p.n_free_out = free_now - n_new;
+    *p.status = bad;
+  }
+}
+
+// The way back.  A sequence's pages go back behind those of the sequences after it, its last page first: the reverse of taking them.
+__global__ void __launch_bounds__(kTableThreads) shrink_kernel(const TableParams p) {
+  extern __shared__ int sm[];
+  int* len = sm;
+  int* left = len + p.n_seq;
+  int* page0 = left + p.n_seq;               // pages that the sequences before it give back
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, per = (p.n_seq + kTableThreads - 1) / kTableThreads;
+  const int first = min(tid * per, p.n_seq), last = min(first + per, p.n_seq);
+  const int free_now = *p.n_free, size1 = (1 << p.shift) - 1;
+  long long pages = 0;
+  int bad = 0;
+  for (int b = first; b < last; ++b) {
+    const long long l = p.lens[b];
+    const long long to = max(0ll, l - max(p.change[b], 0));
+    if (l < 0 || ((l + size1) >> p.shift) > p.max_pages) { bad = 1; continue; }
+    len[b] = (int)l;
+    left[b] = (int)to;
+    pages += ((l + size1) >> p.shift) - ((to + size1) >> p.shift);
+  }
+  long long ep, ez, tp, tz;
+  scan2(pages, 0, ep, ez, tp, tz);
+  bad = __syncthreads_or(bad);
+  if (free_now < 0 || free_now + tp > p.n_pages) bad = 1;
+  if (!bad)
+    for (int b = first; b < last; ++b) {
+      page0[b] = (int)ep;
+      ep += ((len[b] + size1) >> p.shift) - ((left[b] + size1) >> p.shift);
+    }
+  __syncthreads();
+  const int n_back = bad ? 0 : (int)tp;
+  const int stride = kTableThreads * cluster_size();
+  for (int k = cluster_rank() * kTableThreads + tid; k < n_back; k += stride) {
+    const int b = last_at_most(page0, 0, p.n_seq - 1, k);
+    const int place = ((left[b] + size1) >> p.shift) + (k - page0[b]);
+    // k counts upwards over sequences and places; the list's top is the first of them
+    p.free_list[free_now + (n_back - 1 - k)] = p.table[(int64_t)b * p.max_pages + place];
+  }
+  if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();
+  if (cluster_rank() != 0) return;
+  for (int b = tid; b < p.n_seq; b += kTableThreads) {
+    if (!bad) p.lens_out[b] = left[b];
+    else if (p.lens_out != p.lens) p.lens_out[b] = p.lens[b];
+  }
+  if (tid == 0) {
+    *p.n_free_out = free_now + n_back;
+    if (bad) atomicExch(p.dev_err, kv4::kErrFree);
+  }
+}
+
+struct StoreParams {
+  void *k, *v;                               // append reads them, read writes them
+  int64_t k_stride, v_stride;                // elements between rows
+  int rows, heads, D, shift, n_pages;
+  const int* slots;
+  uint8_t* pages;
+  int* dev_err;
+};
+
+template <typename T> struct Pair;           // two neighbouring features
+template <> struct Pair<float> {
+  static __device__ __forceinline__ float2 load(const float* p) { return *reinterpret_cast<const float2*>(p); }
+  static __device__ __forceinline__ void store(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
+};
+template <> struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 load(const __nv_bfloat16* p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p)); }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y); }
+};
+
+// n of one value: rint of the float32 quotient, 0..15
+__device__ __forceinline__ uint32_t level(float x, float m, float s) {
+  return s > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x - m, s)), 0.f), 15.f) : 0u;
+}
+
+// Eight lanes per row, side, head and group; lane (tile, t) has features 16 tile + 2t, 2t + 1, 2t + 8, 2t + 9, which are two bytes of either form.
+template <typename T>
+__global__ void __launch_bounds__(256) append_kernel(const StoreParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int NG = kv4::groups(p.D);
+  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 3;
+  const int l8 = threadIdx.x & 7, tile = l8 >> 2, t = l8 & 3;
+  const int64_t per_row = 2ll * p.heads * NG;
+  const int64_t row = task / per_row;
+  const int rest = (int)(task - row * per_row), side = rest / (p.heads * NG), head = rest / NG % p.heads, g = rest % NG;
+  const bool there = row < p.rows;
+  const int slot = there ? p.slots[row] : -1;
+  float2 a = make_float2(0.f, 0.f), b = a;
+  if (there) {
+    const T* x = reinterpret_cast<const T*>(side ? p.v : p.k) + row * (side ? p.v_stride : p.k_stride) + head * p.D + g * 32 + tile * 16 + 2 * t;
+    a = Pair<T>::load(x);
+    b = Pair<T>::load(x + 8);
+  }
+  float lo = fminf(fminf(a.x, a.y), fminf(b.x, b.y)), hi = fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
+  bool odd = a.x != a.x || a.y != a.y || b.x != b.x || b.y != b.y;
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    odd = __shfl_xor_sync(0xffffffffu, (int)odd, off) | (int)odd;
+  }
+  if (!there || slot < 0) return;
+  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); return; }
+  __half m = __float2half_rn(lo), s = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+  if (odd || __hisinf(m) || __hisinf(s) || __hisnan(s)) m = s = __ushort_as_half(0x7fff);   // a group without a 4-bit form reads back as NaN
+  const float mf = __half2float(m), sf = __half2float(s);
+  const uint32_t e0 = level(a.x, mf, sf) | level(b.x, mf, sf) << 4, e1 = level(a.y, mf, sf) | level(b.y, mf, sf) << 4;
+  const int key = slot & 15;
+  uint8_t* block = p.pages + (((int64_t)(slot >> p.shift) * p.heads + head) * (1 << (p.shift - 4)) + ((slot & ((1 << p.shift) - 1)) >> 4)) * kv4::block_bytes(p.D);
+  uint8_t* data = block + (side ? 8 * p.D : 0);
+  const int d = g * 32 + tile * 16 + 2 * t;
+  data[side ? kv4::value_byte(key, d) : kv4::key_byte(key, d)] = (uint8_t)e0;
+  data[side ? kv4::value_byte(key, d + 1) : kv4::key_byte(key, d + 1)] = (uint8_t)e1;
+  if (l8 == 0) {
+    __half* meta = reinterpret_cast<__half*>(block + 16 * p.D) + side * p.D;
+    const int at = side ? kv4::value_meta(key, g) : kv4::key_meta(key, g);
+    meta[at] = s;
+    meta[p.D / 2 + at] = m;
+  }
+}
+
+// The same lanes the other way.
+template <typename T>
+__global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int NG = kv4::groups(p.D);
+  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 3;
+  const int l8 = threadIdx.x & 7, tile = l8 >> 2, t = l8 & 3;
+  const int64_t per_row = 2ll * p.heads * NG;
+  const int64_t row = task / per_row;
+  if (row >= p.rows) return;
+  const int rest = (int)(task - row * per_row), side = rest / (p.heads * NG), head = rest / NG % p.heads, g = rest % NG;
+  const int slot = p.slots[row];
+  if (slot < 0) return;
+  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); return; }
+  const int key = slot & 15;
+  const uint8_t* block = p.pages + (((int64_t)(slot >> p.shift) * p.heads + head) * (1 << (p.shift - 4)) + ((slot & ((1 << p.shift) - 1)) >> 4)) * kv4::block_bytes(p.D);
+  const uint8_t* data = block + (side ? 8 * p.D : 0);
+  const int d = g * 32 + tile * 16 + 2 * t;
+  const uint32_t e0 = data[side ? kv4::value_byte(key, d) : kv4::key_byte(key, d)], e1 = data[side ? kv4::value_byte(key, d + 1) : kv4::key_byte(key, d + 1)];
+  const __half* meta = reinterpret_cast<const __half*>(block + 16 * p.D) + side * p.D;
+  const int at = side ? kv4::value_meta(key, g) : kv4::key_meta(key, g);
+  const float s = __half2float(meta[at]), m = __half2float(meta[p.D / 2 + at]);
+  T* x = reinterpret_cast<T*>(side ? p.v : p.k) + row * (side ? p.v_stride : p.k_stride) + head * p.D + d;
+  Pair<T>::store(x, make_float2(fmaf((float)(e0 & 15), s, m), fmaf((float)(e1 & 15), s, m)));
+  Pair<T>::store(x + 8, make_float2(fmaf((float)(e0 >> 4), s, m), fmaf((float)(e1 >> 4), s, m)));
+}
+
+template <typename K>
+cudaError_t launch_cluster(K kernel, int ctas, size_t smem, cudaStream_t st, const TableParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kTableThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+int32_t check_tables(const char* who, int n_seq, int page, int max_pages, int n_pages) {
+  LMB_REQUIRE(n_seq >= 1 && n_seq <= kMaxSeqs, "%s: %d sequences (1 to %d)", who, n_seq, kMaxSeqs);
+  LMB_REQUIRE(max_pages >= 1, "%s: block tables of %d pages", who, max_pages);
+  return kv4::check_cache(who, 1, 32, n_pages, page);
+}
+
+int32_t store_params(const char* who, Ctx* ctx, int32_t dtype, const void* k, const void* v, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t heads, int32_t D,
+                     const int32_t* slots, const void* pages, int32_t n_pages, int32_t page, StoreParams* p) {
+  LMB_REQUIRE(dtype == LMB200_F32 || dtype == LMB200_BF16, "%s: dtype %d", who, dtype);
+  LMB_TRY(kv4::check_cache(who, heads, D, n_pages, page));
+  LMB_REQUIRE(rows >= 0, "%s: %d rows", who, rows);
+  LMB_REQUIRE(rows == 0 || (k && v && slots && pages), "%s: null pointer", who);
+  const int64_t width = (int64_t)heads * D;
+  LMB_REQUIRE(k_stride >= width && v_stride >= width, "%s: row strides %lld and %lld for rows of %lld elements", who, (long long)k_stride, (long long)v_stride, (long long)width);
+  const int vec = dtype == LMB200_F32 ? 4 : 8;
+  LMB_REQUIRE(k_stride % vec == 0 && v_stride % vec == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (uintptr_t)pages % 16 == 0,
+              "%s: rows and pages must start on 16-byte boundaries", who);
+  p->k = const_cast<void*>(k); p->v = const_cast<void*>(v);
+  p->k_stride = k_stride; p->v_stride = v_stride;
+  p->rows = rows; p->heads = heads; p->D = D; p->shift = kv4::page_shift(page); p->n_pages = n_pages;
+  p->slots = slots;
+  p->pages = static_cast<uint8_t*>(const_cast<void*>(pages));
+  p->dev_err = ctx->dev_err;
+  return LMB200_OK;
+}
+
+template <typename K>
+int32_t launch_store(Ctx* ctx, K kernel, const StoreParams& p) {
+  const int64_t threads = (int64_t)p.rows * 2 * p.heads * kv4::groups(p.D) * 8;
+  LMB_REQUIRE(ceil_div(threads, 256) <= INT_MAX, "kv4: %d rows of %d heads are too many for one call", p.rows, p.heads);
+  LMB_CUDA(launch_k_opt(false, kernel, dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, ctx->stream, p));
+  ctx->launches++;
+  return LMB200_OK;
+}
+
+}  // namespace
+
+int32_t paged_configure() {
+  const int smem = kMaxSeqs * 3 * 4;
+  LMB_CUDA(cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  LMB_CUDA(cudaFuncSetAttribute(shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  return LMB200_OK;
+}
+
+}  // namespace lmb
+
+using namespace lmb;
+
+extern "C" int32_t lmb200_kv4_page_bytes(int32_t page_size, int32_t n_kv_heads, int32_t head_dim, int64_t* bytes) {
+  LMB_REQUIRE(bytes, "kv4_page_bytes: null argument");
+  LMB_TRY(kv4::check_cache("kv4_page_bytes", n_kv_heads, head_dim, 1, page_size));
+  *bytes = (int64_t)n_kv_heads * (page_size / 16) * kv4::block_bytes(head_dim);
+  return LMB200_OK;
+}
+
+extern "C" int32_t lmb200_kv_reserve(lmb200_ctx h, int32_t n_seq, int32_t page_size, int32_t max_pages, int32_t n_pages, int32_t rows, const int32_t* lens,
+                                     const int32_t* add, int32_t* table, const int32_t* free_list, const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out,
+                                     int32_t* cu_rows, int32_t* slots, int32_t* status) {
+  Ctx* ctx = ctx_from(h);
+  if (!ctx) return LMB200_EINVAL;
+  LMB_TRY(check_tables("kv_reserve", n_seq, page_size, max_pages, n_pages));
+  LMB_REQUIRE(rows >= 0, "kv_reserve: %d rows", rows);
+  LMB_REQUIRE(lens && add && table && free_list && n_free && lens_out && n_free_out && cu_rows && status && (slots || rows == 0), "kv_reserve: null pointer");
+  LMB_CUDA(cudaSetDevice(ctx->device));
+  TableParams p = {n_seq, kv4::page_shift(page_size), max_pages, n_pages, rows, lens, add, n_free, table, const_cast<int32_t*>(free_list),
+                   lens_out, n_free_out, cu_rows, slots, status, ctx->dev_err};
+  LMB_CUDA(launch_cluster(reserve_kernel, n_seq > 512 || rows > 4096 ? 8 : 1, (size_t)n_seq * 12, ctx->stream, p));
+  ctx->launches++;
+  return LMB200_OK;
+}
+
+extern "C" int32_t lmb200_kv_shrink(lmb200_ctx h, int32_t n_seq, int32_t page_size, int32_t max_pages, int32_t n_pages, const int32_t* lens, const int32_t* drop,
+                                    const int32_t* table, int32_t* free_list, const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out) {
+  Ctx* ctx = ctx_from(h);
+  if (!ctx) return LMB200_EINVAL;
+  LMB_TRY(check_tables("kv_shrink", n_seq, page_size, max_pages, n_pages));
+  LMB_REQUIRE(lens && drop && table && free_list && n_free && lens_out && n_free_out, "kv_shrink: null pointer");
+  LMB_CUDA(cudaSetDevice(ctx->device));
+  TableParams p = {n_seq, kv4::page_shift(page_size), max_pages, n_pages, 0, lens, drop, n_free, const_cast<int32_t*>(table), free_list,
+                   lens_out, n_free_out, nullptr, nullptr, nullptr, ctx->dev_err};
+  LMB_CUDA(launch_cluster(shrink_kernel, n_seq > 512 ? 8 : 1, (size_t)n_seq * 12, ctx->stream, p));
+  ctx->launches++;
+  return LMB200_OK;
+}
+
+extern "C" int32_t lmb200_kv4_append(lmb200_ctx h, int32_t dtype, const void* k, const void* v, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads,
+                                     int32_t head_dim, const int32_t* slots, void* pages, int32_t n_pages, int32_t page_size) {
+  Ctx* ctx = ctx_from(h);
+  if (!ctx) return LMB200_EINVAL;
+  StoreParams p;
+  LMB_TRY(store_params("kv4_append", ctx, dtype, k, v, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
+  if (rows == 0) return LMB200_OK;
+  LMB_CUDA(cudaSetDevice(ctx->device));
+  return dtype == LMB200_F32 ? launch_store(ctx, append_kernel<float>, p) : launch_store(ctx, append_kernel<__nv_bfloat16>, p);
+}
+
+extern "C" int32_t lmb200_kv4_read(lmb200_ctx h, int32_t dtype, void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads,
+                                   int32_t head_dim, const int32_t* slots, const void* pages, int32_t n_pages, int32_t page_size) {
+  Ctx* ctx = ctx_from(h);
+  if (!ctx) return LMB200_EINVAL;
+  StoreParams p;
+  LMB_TRY(store_params("kv4_read", ctx, dtype, k_out, v_out, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
+  if (rows == 0) return LMB200_OK;
+  LMB_CUDA(cudaSetDevice(ctx->device));
+  return dtype == LMB200_F32 ? launch_store(ctx, read_kernel<float>, p) : launch_store(ctx, read_kernel<__nv_bfloat16>, p);
+}
