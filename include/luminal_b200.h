@@ -600,7 +600,7 @@ int32_t lmb200_decode_attention_noalloc(lmb200_ctx ctx, int32_t dtype, const voi
  * lmb200_kv4_page_bytes bytes a page, [kv head][token / 16][20 head_dim bytes]; inside a block of 16 tokens, with g = d / 32 and t16 = token % 16:
  *   bytes 0 .. 8 D - 1       keys: 4-byte words [g][t16 % 8][d % 8 / 2][d / 16 % 2], byte 2 (d % 2) + t16 / 8 of the word, low half if d % 16 < 8, else high half
  *   bytes 8 D .. 16 D - 1    values: 4-byte words [g][d % 8][t16 % 8 / 2][d / 16 % 2], byte 2 (t16 % 2) + t16 / 8 of the word, low half if d % 16 < 8, else high half
- *   then float16, D each     key s and key m [g][t16 % 8][t16 / 8]; value s and value m [g][t16 % 8 / 2][t16 / 8][t16 % 2]
+ *   then float16, D / 2 each key s, key m [g][t16 % 8][t16 / 8], value s, value m [g][t16 % 8 / 2][t16 / 8][t16 % 2]
  * A slot is page * page_size + place in the page.  The places of a cache that no call has written are the caller's (zeros read back as 0).
  *
  * A slot or a table entry outside the cache, or row offsets outside the rows, touch no memory: they are left out and the next synchronising call

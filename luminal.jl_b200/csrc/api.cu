@@ -20,6 +20,7 @@ namespace lmb {
 int32_t flash_tc_configure();
 int32_t flash_tc_f32_configure();
 int32_t paged_configure();
+int32_t kv4_attention_configure();
 
 static thread_local char g_err[1024] = "";
 
@@ -337,6 +338,7 @@ extern "C" int32_t lmb200_init(int32_t device, lmb200_ctx* out) {
   if (rc == LMB200_OK) rc = prefill_configure();
   if (rc == LMB200_OK) rc = layered_configure();
   if (rc == LMB200_OK) rc = paged_configure();
+  if (rc == LMB200_OK) rc = kv4_attention_configure();
   if (rc != LMB200_OK) { cudaFree(c->dev_broken); cudaFreeHost(c->dev_err); cudaStreamDestroy(c->own_stream); delete c; return rc; }
   *out = reinterpret_cast<lmb200_ctx>(c);
   return LMB200_OK;

@@ -1,103 +1,29 @@
-// Attention over the 4-bit paged cache (lmb200_kv4_attention).
-#include <math_constants.h>
+// Attention over the 4-bit paged cache (lmb200_kv4_attention): the choice of a variant and its launch.
+#include <algorithm>
 
-#include "kv4.cuh"
-#include "pdl.cuh"
+#include "kv4_attention.cuh"
 
 namespace lmb {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kThreads = 128;
+// The grid of a variant: every CTA that fits on the GPU.  CTAs do not wait for one another, so fewer may run at a time.
+int grid_of(const Ctx* ctx, const kv4::Variant* v) { return std::min(ctx->sm_count * std::max(1, v->ctas_per_sm), kv4::kCounterBytes / 4); }
 
-struct Kv4Params {
-  const void* q;
-  void* out;
-  int64_t q_stride, out_stride;
-  int rows, n_seq, max_pages, n_pages, shift, heads, G, D, window;
-  float scale;
-  const int *cu_rows, *lens, *table;
-  const uint8_t* pages;
-  int* dev_err;
-};
-
-// One CTA per row and query head, its threads over keys for the scores and over features for the values.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const Kv4Params p) {
-  __shared__ float q[256], w[kThreads], red[8];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int r = blockIdx.x, hq = blockIdx.y, h = hq / p.G, tid = threadIdx.x, D = p.D, NG = kv4::groups(D);
-  if (r == 0 && hq == 0)                     // one CTA looks the offsets and lengths over
-    for (int b = tid; b < p.n_seq; b += kThreads)
-      if (p.cu_rows[b] < 0 || p.cu_rows[b + 1] < p.cu_rows[b] || p.cu_rows[b + 1] > p.rows || p.lens[b] < 0 || p.lens[b] > p.max_pages << p.shift)
-        atomicExch(p.dev_err, kv4::kErrPage);
-  int lo = 0, hi = p.n_seq;
-  while (lo < hi) {                          // the first sequence that ends behind row r
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_rows[mid + 1] <= r) lo = mid + 1; else hi = mid;
-  }
-  if (lo >= p.n_seq || r < p.cu_rows[lo]) return;
-  const int b = lo, size1 = (1 << p.shift) - 1;
-  const int len = min(max(p.lens[b], 0), p.max_pages << p.shift);
-  const int position = len - (p.cu_rows[b + 1] - r);
-  const int from = p.window > 0 ? max(0, position - p.window + 1) : 0;
-  const T* qr = reinterpret_cast<const T*>(p.q) + r * p.q_stride + hq * D;
-  for (int d = tid; d < D; d += kThreads) q[d] = to_f32(qr[d]) * p.scale * kLog2e;
-  float M = -CUDART_INF_F, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int k0 = from; k0 <= position; k0 += kThreads) {
-    __syncthreads();
-    const int key = k0 + tid;
-    float s = -CUDART_INF_F;
-    const int n = min(kThreads, position + 1 - k0);
-    if (tid < n) {
-      const int page = p.table[(int64_t)b * p.max_pages + (key >> p.shift)];
-      if ((unsigned)page < (unsigned)p.n_pages) {
-        const uint8_t* block = p.pages + (((int64_t)page * p.heads + h) * (1 << (p.shift - 4)) + ((key & size1) >> 4)) * kv4::block_bytes(D);
-        const __half* meta = reinterpret_cast<const __half*>(block + 16 * D);
-        s = 0.f;
-        for (int d = 0; d < D; ++d) {
-          const int n4 = block[kv4::key_byte(key & 15, d)] >> ((d & 8) ? 4 : 0) & 15, at = kv4::key_meta(key & 15, d >> 5);
-          s = fmaf(q[d], fmaf((float)n4, __half2float(meta[at]), __half2float(meta[D / 2 + at])), s);
-        }
-      } else {
-        atomicExch(p.dev_err, kv4::kErrPage);
-      }
-    }
-    float top = s;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    if ((tid & 31) == 0) red[tid >> 5] = top;
-    __syncthreads();
-    const float Mn = fmaxf(M, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]))), Mu = Mn == -CUDART_INF_F ? 0.f : Mn;
-    const float fade = exp2f(M - Mu), e = exp2f(s - Mu);
-    w[tid] = e;
-    float sum = e;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if ((tid & 31) == 0) red[4 + (tid >> 5)] = sum;
-    __syncthreads();
-    l = l * fade + ((red[4] + red[5]) + (red[6] + red[7]));
-    M = Mn;
-    for (int i = 0, d = tid; d < D; ++i, d += kThreads) {
-      float o = (i ? o1 : o0) * fade;
-      for (int j = 0; j < n; ++j) {
-        if (w[j] == 0.f) continue;           // also keys of a page that is not there
-        const int kk = k0 + j;
-        const int page = p.table[(int64_t)b * p.max_pages + (kk >> p.shift)];
-        const uint8_t* block = p.pages + (((int64_t)page * p.heads + h) * (1 << (p.shift - 4)) + ((kk & size1) >> 4)) * kv4::block_bytes(D);
-        const __half* meta = reinterpret_cast<const __half*>(block + 16 * D) + D;
-        const int n4 = block[8 * D + kv4::value_byte(kk & 15, d)] >> ((d & 8) ? 4 : 0) & 15, at = kv4::value_meta(kk & 15, d >> 5);
-        o = fmaf(w[j], fmaf((float)n4, __half2float(meta[at]), __half2float(meta[D / 2 + at])), o);
-      }
-      if (i) o1 = o; else o0 = o;
-    }
-  }
-  T* out = reinterpret_cast<T*>(p.out) + r * p.out_stride + hq * D;
-  for (int i = 0, d = tid; d < D; ++i, d += kThreads) out[d] = from_f32<T>(l > 0.f || l != l ? (i ? o1 : o0) / l : 0.f);
+int64_t workspace_bytes_of(const Ctx* ctx, int D) {
+  int64_t most = 0;
+  for (int f32 = 0; f32 < 2; ++f32)
+    for (int nt = 1; nt <= kv4::most_tiles(f32, kv4::groups(D)); ++nt)
+      most = std::max<int64_t>(most, (int64_t)grid_of(ctx, f32 ? kv4::variant_f32(kv4::groups(D), nt) : kv4::variant_bf16(kv4::groups(D), nt)) * 2 * (8 * nt) * (D + 2) * 4);
+  return kv4::kCounterBytes + most;
 }
 
 }  // namespace
+
+int32_t kv4_attention_configure() {
+  LMB_TRY(kv4::configure_bf16());
+  return kv4::configure_f32();
+}
+
 }  // namespace lmb
 
 using namespace lmb;
@@ -107,7 +33,7 @@ extern "C" int32_t lmb200_kv4_attention_workspace(lmb200_ctx h, int32_t head_dim
   if (!ctx) return LMB200_EINVAL;
   LMB_REQUIRE(bytes, "kv4_attention_workspace: null argument");
   LMB_TRY(kv4::check_cache("kv4_attention_workspace", 1, head_dim, 1, 16));
-  *bytes = 16;
+  *bytes = workspace_bytes_of(ctx, head_dim);
   return LMB200_OK;
 }
 
@@ -129,16 +55,33 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   const int vec = dtype == LMB200_F32 ? 4 : 8;
   LMB_REQUIRE(q_stride % vec == 0 && out_stride % vec == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)pages % 16 == 0 &&
                   (uintptr_t)workspace % 16 == 0, "kv4_attention: rows, pages and workspace must start on 16-byte boundaries");
-  int64_t need = 0;
-  LMB_TRY(lmb200_kv4_attention_workspace(h, head_dim, &need));
+  const int64_t need = workspace_bytes_of(ctx, head_dim);
   LMB_REQUIRE(workspace_bytes >= need, "kv4_attention: a workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
   if (rows == 0) return LMB200_OK;
+  // Query rows of one kv head that share a pass over its keys, in tiles of 8: what a sequence has on average (only the device knows each one's), as far as registers go.
+  const bool f32 = dtype == LMB200_F32;
+  const int NG = kv4::groups(head_dim);
+  const int64_t each = ceil_div(ceil_div(rows, n_seq) * group, 8);
+  const int NT = (int)std::min<int64_t>(each, kv4::most_tiles(f32, NG));
+  const kv4::Variant* v = f32 ? kv4::variant_f32(NG, NT) : kv4::variant_bf16(NG, NT);
+  // units of work are counted in 32 bits
+  const int64_t tiles = ceil_div((int64_t)rows * group, 8 * NT) + std::min(n_seq, rows), units = ceil_div((int64_t)max_pages * page_size, kv4::kUnit) + 1;
+  LMB_REQUIRE(tiles * n_kv_heads <= UINT32_MAX / units, "kv4_attention: %d rows of %d heads over %d pages are too many for one call", rows, n_kv_heads * group, max_pages);
   LMB_CUDA(cudaSetDevice(ctx->device));
-  Kv4Params p = {q, out, q_stride, out_stride, rows, n_seq, max_pages, n_pages, kv4::page_shift(page_size), n_kv_heads, group, head_dim, window,
-                 scale, cu_rows, lens, table, static_cast<const uint8_t*>(pages), ctx->dev_err};
-  const dim3 grid((unsigned)rows, (unsigned)(n_kv_heads * group));
-  if (dtype == LMB200_F32) LMB_CUDA(launch_k_opt(false, kv4_attention_kernel<float>, grid, dim3(kThreads), 0, ctx->stream, p));
-  else LMB_CUDA(launch_k_opt(false, kv4_attention_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, ctx->stream, p));
+  const int grid = (int)std::min<int64_t>(grid_of(ctx, v), tiles * n_kv_heads * units);
+  kv4::Params p = {};
+  p.q = q; p.out = out; p.q_stride = q_stride; p.out_stride = out_stride;
+  p.rows = rows; p.n_seq = n_seq; p.max_pages = max_pages; p.n_pages = n_pages; p.shift = kv4::page_shift(page_size);
+  p.heads = n_kv_heads; p.G = group; p.window = window;
+  p.scale = scale * 1.4426950408889634f;
+  p.cu_rows = cu_rows; p.lens = lens; p.table = table;
+  p.pages = static_cast<const uint8_t*>(pages);
+  p.dev_err = ctx->dev_err;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.counters = reinterpret_cast<unsigned*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + kv4::kCounterBytes);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)grid * 2 * 8 * NT * head_dim);
+  LMB_CUDA(launch_k_opt(false, v->kernel, dim3((unsigned)grid), dim3(kv4::kThreads), (size_t)v->smem + (n_seq + 1) * 4, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
 }
