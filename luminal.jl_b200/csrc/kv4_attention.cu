@@ -7,14 +7,14 @@ namespace lmb {
 namespace {
 
 // The grid of a variant: every CTA that fits on the GPU.  CTAs do not wait for one another, so fewer may run at a time.
-int grid_of(const Ctx* ctx, const kv4::Variant* v) { return std::min(ctx->sm_count * std::max(1, v->ctas_per_sm), kv4::kCounterBytes / 4); }
+int grid_of(const Ctx* ctx, const kv4::Variant* v) { return std::min(ctx->sm_count * std::max(1, v->ctas_per_sm), kv4::kMostShares); }
 
 int64_t workspace_bytes_of(const Ctx* ctx, int D) {
   int64_t most = 0;
   for (int f32 = 0; f32 < 2; ++f32)
     for (int nt = 1; nt <= kv4::most_tiles(f32, kv4::groups(D)); ++nt)
       most = std::max<int64_t>(most, (int64_t)grid_of(ctx, f32 ? kv4::variant_f32(kv4::groups(D), nt) : kv4::variant_bf16(kv4::groups(D), nt)) * 2 * (8 * nt) * (D + 2) * 4);
-  return kv4::kCounterBytes + most;
+  return kv4::kCounters * 4 + most;
 }
 
 }  // namespace
@@ -79,9 +79,9 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   p.dev_err = ctx->dev_err;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counters = reinterpret_cast<unsigned*>(ws);
-  p.part_o = reinterpret_cast<float*>(ws + kv4::kCounterBytes);
+  p.part_o = reinterpret_cast<float*>(ws + kv4::kCounters * 4);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)grid * 2 * 8 * NT * head_dim);
-  LMB_CUDA(launch_k_opt(false, v->kernel, dim3((unsigned)grid), dim3(kv4::kThreads), (size_t)v->smem + (n_seq + 1) * 4, ctx->stream, p));
+  LMB_CUDA(launch_k_opt(false, v->kernel, dim3((unsigned)grid), dim3(kv4::kThreads), (size_t)v->smem + kv4::seq_bytes(n_seq), ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
 }

@@ -9,13 +9,11 @@
 // are cut off, not rounded: 3.4e-5 of the result as subnormals in one sum.  Both products are mma.sync m16n8k16 with keys or features as the 16 rows and up to 8 query rows of one kv head as columns, because a decoding
 // step has 1 to 8 of them: on tcgen05 M would be padded to 128, and the 4-bit operand would have to be widened through shared memory instead of in registers.
 //
-// Work.  Units of 128 keys of all (sequence, row tile, kv head) triples in a row are cut into equal shares, one per CTA, whatever the sequences' lengths, so a long
-// sequence among short ones is shared by many CTAs.  Each of a CTA's four warps takes 32 keys of a unit through a ring of bulk copies of its own.  Where
-// a triple is shared, its CTAs leave partial sums and the last one to finish joins them.
+// Work.  Units of 128 keys of all (sequence, row tile, kv head) triples in a row are cut into equal shares whatever the sequences' lengths, so a long sequence among short ones
+// is shared by many CTAs.  Each of a CTA's four warps takes 32 keys of a unit through a ring of bulk copies of its own, which is filled with the next triple's keys while the present
+// one's sums are joined.  Where a triple is cut, its shares leave partial sums and the last one to finish joins them (many: in groups first).
 #pragma once
 #include <math_constants.h>
-
-#include <type_traits>
 
 #include "kv4.cuh"
 #include "pdl.cuh"
@@ -24,7 +22,8 @@
 namespace lmb {
 namespace kv4 {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kUnit = 128, kMaxSeqs = 8192, kCounterBytes = 8192;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kUnit = 128, kMaxSeqs = 8192;
+constexpr int kCounters = 4096, kMostShares = kCounters / 2, kJoin = 16;
 
 struct Params {
   const void* q;
@@ -35,10 +34,13 @@ struct Params {
   const int *cu_rows, *lens, *table;
   const uint8_t* pages;
   int* dev_err;
-  unsigned* counters;                        // [grid], zero between calls
-  float2* part_ml;                           // [grid][2][columns]: maximum (log2) and sum
-  float* part_o;                             // [grid][2][columns][D]
+  unsigned* counters;                        // [kCounters], zero between calls: two per share
+  float2* part_ml;                           // [share][2][columns]: maximum (log2) and sum
+  float* part_o;                             // [share][2][columns][D]
 };
+
+// shared memory that grows with the sequences
+__host__ __device__ constexpr int seq_bytes(int n_seq) { return (2 * n_seq + 1) * 4; }
 
 // One variant: widths of NG groups, NT tiles of 8 query rows.
 struct Variant {
@@ -59,11 +61,10 @@ template <typename T, int NG, int NT> struct Shape {
   static constexpr int kStages = NG == 1 ? 8 : NG == 2 ? 6 : NG == 3 ? 4 : NG <= 5 ? 3 : 2;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kPitch = D + 4;                    // of the joined sums: 2 kPitch = 8 banks
-  static constexpr int kMerge = kWarps * COLS * kPitch * 4;
-  static constexpr int kBig = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kMerge = 2 * COLS * kPitch * 4;
   static constexpr int kQ = 2 * NG * NT * 32 * (kSplit ? 16 : 8);
   static constexpr int kQSum = NT * 32 * 8;
-  static constexpr int kFixed = kBig + kQ + kQSum + COLS * 12 + 2 * kWarps * COLS * 4 + kWarps * kStages * 8 + 64;
+  static constexpr int kFixed = kRing + kMerge + kQ + kQSum + COLS * 16 + 2 * kWarps * COLS * 4 + kWarps * kStages * 8 + 64 + 3 * 96 + kWarps * 16;
 };
 
 __device__ __forceinline__ void mma_half(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -71,13 +72,25 @@ __device__ __forceinline__ void mma_half(float (&c)[4], uint32_t a0, uint32_t a1
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// c += a b with b = hi + lo
+// c = a b
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// c (+)= a b with b = hi + lo
+template <bool kFirst>
 __device__ __forceinline__ void mma_split(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t h0, uint32_t h1, uint32_t l0, uint32_t l1) {
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  mma_half(x, a0, a1, a2, a3, l0, l1);
+  float x[4];
+  mma_first(x, a0, a1, a2, a3, l0, l1);
   mma_half(x, a0, a1, a2, a3, h0, h1);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) c[k] += x[k];
+  for (int k = 0; k < 4; ++k) c[k] = kFirst ? x[k] : c[k] + x[k];
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t d;
@@ -98,12 +111,21 @@ template <bool kNormal> __device__ __forceinline__ uint32_t numbers(uint32_t x, 
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
-// Where a unit of work lies.
+// What a warp works on, and where it stands in its CTA's share: in shared memory, because the pass over the keys has no registers to spare.  The warps of a CTA all write the
+// same segment, into one of three places in turn.
 struct Segment {
-  int b, tile, head;                         // triple
-  int rows0, T, len;                         // the sequence's first row, its rows, its tokens
-  int first_unit, n_units;                   // of the triple: keys kUnit first_unit ..
   int64_t item0;                             // the triple's first unit in the common order
+  const int* row_table;
+  const uint8_t* head_pages;                 // of its kv head in page 0
+  int tile, head, valid, pad;                // valid: query rows of the tile
+  int rows0, position0;                      // of the sequence's first new token
+  int n_units, from_unit, to_unit;           // of the triple: units [from_unit, to_unit)
+  int first_block, highest, lowest;          // keys that some row sees
+  int all_from, all_to;                      // keys that all rows see
+};
+struct Walk {
+  int64_t u;                                 // first unit that is left of the share
+  int b, pad;                                // its sequence
 };
 
 __device__ __forceinline__ int row_tiles(int T, int G, int cols) { return (T * G + cols - 1) / cols; }
@@ -116,52 +138,52 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
   constexpr int BK = NT <= 2 ? 2 : 1;        // blocks of 16 keys whose scores are in registers at once
   constexpr float kPScale = 7.f;             // weights are 2^7 p at the maximum, up to 2^15 while it lags
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* ring = smem;
-  float* merge = reinterpret_cast<float*>(smem);
-  uint8_t* at = smem + S::kBig;
+  uint8_t* at = smem;
+  uint8_t* my_ring = at + (threadIdx.x >> 5) * kStages * S::kStageBytes; at += S::kRing;
+  float* merge = reinterpret_cast<float*>(at); at += S::kMerge;
   uint32_t* qfrag = reinterpret_cast<uint32_t*>(at); at += S::kQ;
   uint2* qsum = reinterpret_cast<uint2*>(at); at += S::kQSum;
-  uint64_t* full = reinterpret_cast<uint64_t*>(at); at += kWarps * kStages * 8;
+  uint64_t* my_full = reinterpret_cast<uint64_t*>(at) + (threadIdx.x >> 5) * kStages; at += kWarps * kStages * 8;
   float* col_scale = reinterpret_cast<float*>(at); at += COLS * 4;
   int* col_end = reinterpret_cast<int*>(at); at += COLS * 4;
   int* col_from = reinterpret_cast<int*>(at); at += COLS * 4;
+  unsigned* col_top = reinterpret_cast<unsigned*>(at); at += COLS * 4;
   float* warp_m = reinterpret_cast<float*>(at); at += kWarps * COLS * 4;
   float* warp_l = reinterpret_cast<float*>(at); at += kWarps * COLS * 4;
-  int* shared_word = reinterpret_cast<int*>(at); at += 64;
+  int* shared_word = reinterpret_cast<int*>(at); at += 64;  // 0..3 sums of warps, 4 the last one's flag
+  Segment* segments = reinterpret_cast<Segment*>(at); at += 3 * 96;
+  Walk* walk = reinterpret_cast<Walk*>(at) + (threadIdx.x >> 5); at += kWarps * 16;
   unsigned* before = reinterpret_cast<unsigned*>(at);      // [n_seq + 1] units of the sequences before
+  int* seq_len = reinterpret_cast<int*>(before + p.n_seq + 1);           // [n_seq] their tokens
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  for (int i = tid; i < kWarps * kStages; i += kThreads) tc::mbar_init(full + i, 1);
+  if (lane < kStages) tc::mbar_init(my_full + lane, 1);
   tc::mbar_init_fence();
+  if (tid < COLS) col_top[tid] = 0;
+  for (int i = tid; i < NT * 32; i += kThreads) qsum[i] = make_uint2(0, 0);               // groups that are not there stay 0
   pdl_launch_dependents();
   pdl_wait();
 
   // units of every sequence
-  const int capacity = p.max_pages << p.shift;
-  auto look_at = [&](int b, int& r0, int& T_, int& len) {
-    r0 = p.cu_rows[b];
-    const int r1 = p.cu_rows[b + 1];
-    len = p.lens[b];
-    bool bad = len < 0 || len > capacity;
-    len = min(max(len, 0), capacity);
-    T_ = r1 - r0;
-    if (r0 < 0 || r1 < r0 || r1 > p.rows) { bad = true; T_ = 0; }
-    return bad;
-  };
-  auto units_of = [&](int T_, int len, int& first) {
+  auto units_of = [&](int T_, int len, int& first) __attribute__((always_inline)) {
     const int lowest = len - T_;                           // position of the first row
     first = p.window > 0 && lowest - p.window + 1 > 0 ? (lowest - p.window + 1) / kUnit : 0;
     return max(1, (len + kUnit - 1) / kUnit - first);      // a sequence without keys still has rows to write
   };
   {
+    const int capacity = p.max_pages << p.shift;
     const int per = (p.n_seq + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, p.n_seq), b1 = min(b0 + per, p.n_seq);
     unsigned sum = 0;
     bool bad = false;
     for (int b = b0; b < b1; ++b) {
-      int r0, T_, len, first;
-      bad |= look_at(b, r0, T_, len);
+      const int r0 = p.cu_rows[b], r1 = p.cu_rows[b + 1], l = p.lens[b];
+      const int len = min(max(l, 0), capacity);
+      int T_ = r1 - r0, first;
+      bad |= l != len;
+      if (r0 < 0 || r1 < r0 || r1 > p.rows) { bad = true; T_ = 0; }
       const unsigned n = T_ > 0 ? (unsigned)row_tiles(T_, p.G, COLS) * p.heads * units_of(T_, len, first) : 0u;
+      seq_len[b] = len;
       before[b + 1] = n;
       sum += n;
     }
@@ -180,141 +202,303 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
     if (tid == 0) before[0] = 0;
     __syncthreads();
   }
-  const int64_t U = before[p.n_seq], grid = min((int64_t)gridDim.x, U);                  // every CTA that takes part has a unit
-  if ((int64_t)blockIdx.x >= grid) return;
-  int64_t u = U * blockIdx.x / grid;
+  // every CTA that takes part has a share, every share a unit
+  const int64_t U = before[p.n_seq];
+  const int grid = (int)min((int64_t)gridDim.x, U);
+  if ((int)blockIdx.x >= grid) return;
+
+  const int per_page = 1 << (p.shift - 4);
+
+  // the next segment of the CTA's share into *sg; false behind the last
   const int64_t u_end = U * (blockIdx.x + 1) / grid;
-  int b;
+  auto advance = [&](Segment* sg) __attribute__((always_inline)) -> bool {
+    const int64_t u = walk->u;
+    if (u >= u_end) return false;
+    int b = walk->b;
+    while ((int64_t)before[b + 1] <= u) ++b;
+    int first_unit;
+    const int rows0 = p.cu_rows[b], T_ = p.cu_rows[b + 1] - rows0, len = seq_len[b];
+    const int n_units = units_of(T_, len, first_unit);
+    const int triple = (int)(u - before[b]) / n_units, tile = triple / p.heads, head = triple - tile * p.heads;
+    const int64_t item0 = (int64_t)before[b] + (int64_t)triple * n_units;
+    const int valid = min(COLS, T_ * p.G - tile * COLS);                 // query rows of this tile; their positions ascend
+    const int first_pos = len - T_ + tile * COLS / p.G, last_pos = len - T_ + (tile * COLS + valid - 1) / p.G;
+    const int to_unit = (int)min((int64_t)n_units, u_end - item0);
+    __syncwarp();
+    if (lane == 0) {
+      sg->item0 = item0;
+      sg->row_table = p.table + (int64_t)b * p.max_pages;
+      sg->head_pages = p.pages + (int64_t)head * per_page * (640 * NG);
+      sg->tile = tile; sg->head = head; sg->valid = valid;
+      sg->rows0 = rows0; sg->position0 = len - T_;
+      sg->n_units = n_units; sg->from_unit = (int)(u - item0); sg->to_unit = to_unit;
+      sg->first_block = (first_unit + (int)(u - item0)) * (kUnit / 16);
+      sg->highest = max(0, last_pos + 1);
+      sg->lowest = p.window > 0 ? max(0, first_pos - p.window + 1) : 0;
+      sg->all_from = p.window > 0 ? max(0, last_pos - p.window + 1) : 0;
+      sg->all_to = max(0, first_pos + 1);
+      walk->u = item0 + to_unit; walk->b = b;
+    }
+    __syncwarp();
+    return true;
+  };
+
+  // ---- ring: stage j holds this warp's two blocks of unit from_unit + j --------------------------------------------------
+  int slot = 0, ids = -1, ids_next = -1;
+  uint32_t phases = 0, loaded = 0;           // per stage of the ring: parity of its next wait; two bits for the blocks that are there
+  bool dead = false;
+  auto place_of = [&](const Segment* sg, int batch) __attribute__((always_inline)) {       // lane: block lane % 2 of stage 16 batch + lane / 2; -1: not to be read
+    const int j = batch * 16 + (lane >> 1), key = (sg->first_block + 2 * warp + j * (kUnit / 16) + (lane & 1)) * 16;
+    return j < sg->to_unit - sg->from_unit && key < sg->highest && key + 16 > sg->lowest ? key >> p.shift : -1;
+  };
+  auto page_at = [&](const Segment* sg, int batch) __attribute__((always_inline)) {
+    const int place = place_of(sg, batch);
+    return place >= 0 ? sg->row_table[place] : -1;
+  };
+  auto checked = [&](const Segment* sg, int batch, int page) __attribute__((always_inline)) {
+    if ((unsigned)page < (unsigned)p.n_pages) return page;
+    if (place_of(sg, batch) >= 0) atomicExch(p.dev_err, kErrPage);
+    return -1;
+  };
+  auto issue = [&](const Segment* sg, int j, int s) __attribute__((always_inline)) {
+    if (j > 0 && (j & 15) == 0) {
+      ids = checked(sg, j >> 4, ids_next);
+      ids_next = page_at(sg, (j >> 4) + 1);
+    }
+    const int p0 = __shfl_sync(0xffffffffu, ids, (j & 15) * 2), p1 = __shfl_sync(0xffffffffu, ids, (j & 15) * 2 + 1);
+    const uint32_t bits = (p0 >= 0 ? 1u : 0u) | (p1 >= 0 ? 2u : 0u);
+    loaded = (loaded & ~(3u << (2 * s))) | bits << (2 * s);
+    if (bits && lane == 0) {
+      const int inside = (sg->first_block + 2 * warp + j * (kUnit / 16)) & (per_page - 1);
+      const int64_t page_pitch = (int64_t)(p.heads * per_page) * (640 * NG);
+      uint8_t* dst = my_ring + s * S::kStageBytes;
+      const uint8_t* src = sg->head_pages + p0 * page_pitch + inside * (640 * NG);
+      if (bits == 3 && per_page > 1) {                     // neighbours in one page
+        tc::mbar_expect_tx(my_full + s, 2 * 640 * NG);
+        tc::bulk_g2s(dst, src, 2 * 640 * NG, my_full + s);
+      } else {
+        tc::mbar_expect_tx(my_full + s, (bits == 3 ? 2 : 1) * 640 * NG);
+        if (bits & 1) tc::bulk_g2s(dst, src, 640 * NG, my_full + s);
+        if (bits & 2) tc::bulk_g2s(dst + 640 * NG, sg->head_pages + p1 * page_pitch + ((inside + 1) & (per_page - 1)) * (640 * NG), 640 * NG, my_full + s);
+      }
+    }
+  };
+  auto start = [&](const Segment* sg, int page0, int page1) __attribute__((always_inline)) {
+    ids = checked(sg, 0, page0);
+    ids_next = page1;
+    slot = 0;
+    const int n = min(kStages, sg->to_unit - sg->from_unit);
+#pragma unroll 1
+    for (int s = 0; s < n; ++s) issue(sg, s, s);
+  };
+
+  // ---- queries: four threads have a group of a row ---------------------------------------------------------------------------
+  constexpr int kTasks = COLS * NG * 4, kRounds = (kTasks + kThreads - 1) / kThreads;
+  auto load_queries = [&](const Segment* sg, uint4 (&v)[kRounds][kSplit ? 2 : 1]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int task = tid + i * kThreads, c = task / (NG * 4), f = (task - c * (NG * 4)) * 8;
+      v[i][0] = make_uint4(0, 0, 0, 0);
+      if (kSplit) v[i][kSplit ? 1 : 0] = make_uint4(0, 0, 0, 0);
+      if (task < kTasks && c < sg->valid) {
+        const int rho = sg->tile * COLS + c, row = rho / p.G, hq = rho - row * p.G;
+        const T* qr = reinterpret_cast<const T*>(p.q) + (int64_t)(sg->rows0 + row) * p.q_stride + (int64_t)(sg->head * p.G + hq) * D + f;
+        v[i][0] = *reinterpret_cast<const uint4*>(qr);
+        if (kSplit) v[i][kSplit ? 1 : 0] = *reinterpret_cast<const uint4*>(qr + 4);
+      }
+    }
+  };
+  auto feature = [&](const uint4 (&v)[kSplit ? 2 : 1], int k) __attribute__((always_inline)) {
+    if (kSplit) {
+      const uint4& w = v[kSplit ? k >> 2 : 0];
+      return __uint_as_float((k & 3) == 0 ? w.x : (k & 3) == 1 ? w.y : (k & 3) == 2 ? w.z : w.w);
+    }
+    const uint32_t w = (k >> 1) == 0 ? v[0].x : (k >> 1) == 1 ? v[0].y : (k >> 1) == 2 ? v[0].z : v[0].w;
+    return __uint_as_float(k & 1 ? w & 0xffff0000u : w << 16);
+  };
+
+  auto put = [&](const Segment* my, int c, int d, float4 v, float L) __attribute__((always_inline)) {
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;             // a row that sees no key is 0
+    const int rho = my->tile * COLS + c, row = rho / p.G, hq = rho - row * p.G;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(my->rows0 + row) * p.out_stride + (int64_t)(my->head * p.G + hq) * D + d;
+    if (kSplit) {
+      *reinterpret_cast<float4*>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    } else {
+      __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv), y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
+      *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
+    }
+  };
+
+  // The last of the shares that cut a triple joins what all of them left; of more than kJoin + kJoin / 2 the last of every kJoin neighbours first joins theirs.
+  struct Part { int first, count, groups, sa; };           // what a part's counter counts: `count` shares from `first` on; groups > 1: of one of so many groups
+  auto counted = [&](unsigned* counter, int of) __attribute__((always_inline)) {           // thread 0, behind a barrier behind all threads' writes
+    unsigned old;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(counter) : "memory");
+    const bool last = old == (unsigned)of - 1u;
+    if (last) *counter = 0u;
+    shared_word[4] = last;
+  };
+  auto count_part = [&](const Segment* my) __attribute__((always_inline)) {
+    Part q;
+    q.sa = (int)(((my->item0 + 1) * grid - 1) / U);
+    const int n = (int)(((my->item0 + my->n_units) * grid - 1) / U) - q.sa + 1;
+    const bool grouped = n > kJoin + kJoin / 2;
+    const int group = grouped ? ((int)blockIdx.x - q.sa) / kJoin : 0;
+    q.groups = grouped ? (n + kJoin - 1) / kJoin : 1;
+    q.first = q.sa + group * kJoin;
+    q.count = grouped ? min(kJoin, n - group * kJoin) : n;
+    if (tid == 0) counted(p.counters + (grouped ? kMostShares : 0) + q.first, q.count);
+    return q;
+  };
+  // behind the barrier behind count_part
+  auto join_parts = [&](const Segment* my, Part q) __attribute__((always_inline)) {
+    if (!shared_word[4]) return;
+    const int my_valid = my->valid;
+    float* weight = merge;                   // [count][my_valid]
+    int first = q.first, count = q.count, step = 1;
+#pragma unroll 1
+    for (bool done = q.groups == 1;; done = true) {
+      // parts k of `count`, `step` shares apart: to the output, or to the first one's place
+      auto place = [&](int k) __attribute__((always_inline)) { return (int64_t)((first + k * step) * 2 + (first + k * step == q.sa)) * COLS; };
+      for (int c = warp; c < my_valid; c += kWarps) {
+        float top = -CUDART_INF_F, L = 0.f;
+        for (int k = lane; k < count; k += 32) top = fmaxf(top, __ldcg(&p.part_ml[place(k) + c].x));
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        for (int k = lane; k < count; k += 32) {
+          const float2 ml = __ldcg(p.part_ml + place(k) + c);
+          const float f = ml.x == -CUDART_INF_F ? (ml.y != ml.y ? 1.f : 0.f) : exp2_fast(ml.x - top);
+          weight[k * my_valid + c] = f;
+          L = fmaf(ml.y, f, L);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+        if (lane == 0) { warp_m[c] = top; warp_l[c] = L; }
+      }
+      __syncthreads();
+      for (int i = tid; i < my_valid * (D / 4); i += kThreads) {
+        const int c = i / (D / 4), d = (i - c * (D / 4)) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int k0 = 0; k0 < count; k0 += 8) {            // eight loads on their way at a time
+          float4 x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (place(min(k0 + k, count - 1)) + c) * D + d));
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float f = k0 + k < count ? weight[(k0 + k) * my_valid + c] : 0.f;
+            if (f != 0.f) { sum.x = fmaf(x[k].x, f, sum.x); sum.y = fmaf(x[k].y, f, sum.y); sum.z = fmaf(x[k].z, f, sum.z); sum.w = fmaf(x[k].w, f, sum.w); }
+          }
+        }
+        if (done) {
+          put(my, c, d, sum, warp_l[c]);
+        } else {
+          __stcg(reinterpret_cast<float4*>(p.part_o + (place(0) + c) * D + d), sum);
+          if (d == 0) __stcg(p.part_ml + place(0) + c, make_float2(warp_m[c], warp_l[c]));
+        }
+      }
+      __syncthreads();
+      if (done) break;
+      if (tid == 0) counted(p.counters + q.sa, q.groups);
+      __syncthreads();
+      if (!shared_word[4]) break;
+      first = q.sa;
+      count = q.groups;
+      step = kJoin;
+    }
+  };
+
   {
-    int lo = 0, hi = p.n_seq - 1;                          // the last sequence with before[b] <= u
+    const int64_t u = U * blockIdx.x / grid;
+    int lo = 0, hi = p.n_seq - 1;            // the last sequence with before[b] <= u
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if ((int64_t)before[mid] <= u) lo = mid; else hi = mid - 1;
     }
-    b = lo;
+    if (lane == 0) { walk->u = u; walk->b = lo; }
   }
-
-  int slot = 0;                              // ring state, of this warp
-  uint32_t phases = 0;                       // bit s: parity of the next wait on stage s
-  bool dead = false;
-  uint8_t* my_ring = ring + warp * kStages * S::kStageBytes;
-  uint64_t* my_full = full + warp * kStages;
-
-  while (u < u_end) {
-    while ((int64_t)before[b + 1] <= u) ++b;
-    Segment sg;
-    sg.b = b;
-    look_at(b, sg.rows0, sg.T, sg.len);
-    sg.n_units = units_of(sg.T, sg.len, sg.first_unit);
-    const int in_seq = (int)(u - before[b]), triple = in_seq / sg.n_units;
-    sg.tile = triple / p.heads;
-    sg.head = triple - sg.tile * p.heads;
-    sg.item0 = (int64_t)before[b] + (int64_t)triple * sg.n_units;
-    const int from_unit = (int)(u - sg.item0), to_unit = (int)min((int64_t)sg.n_units, u_end - sg.item0);
-    const int valid = min(COLS, sg.T * p.G - sg.tile * COLS);            // query rows of this tile
-    u = sg.item0 + to_unit;
-
-    // ---- queries: MMA operands, sums per group, each row scaled to [2^9, 2^10) --------------------------------------
-    __syncthreads();                         // the previous segment's shared memory is free
-    for (int c = warp; c < COLS; c += kWarps) {
-      const int rho = sg.tile * COLS + c, row = rho / p.G, hq = rho - row * p.G;
-      const T* qr = reinterpret_cast<const T*>(p.q) + (int64_t)(sg.rows0 + row) * p.q_stride + (int64_t)(sg.head * p.G + hq) * D;
-      float v[NG], top = 0.f;
+  __syncwarp();
+  int at_segment = 0;
+  bool more = true, pending = false;         // a part of the segment before this one waits to be counted
+  advance(segments);
+  uint4 v[kRounds][kSplit ? 2 : 1];
+  load_queries(segments, v);
+  start(segments, page_at(segments, 0), page_at(segments, 1));
+  for (;;) {
+    const Segment* sg = segments + at_segment;
+    // ---- queries: MMA operands, sums per group, each row scaled to [2^9, 2^10) ----------------------------------------------
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        v[i] = c < valid ? to_f32(qr[i * 32 + lane]) : 0.f;
-        top = fmaxf(top, fabsf(v[i]));
-      }
+    for (int i = 0; i < kRounds; ++i) {
+      const int task = tid + i * kThreads, c = task / (NG * 4);
+      unsigned top = 0;
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127, -117) : 9;   // 2^(9 - e) stays a float
-      const float up = __uint_as_float((uint32_t)(min(127 + 9 - e, 253)) << 23), down = __uint_as_float((uint32_t)max(127 - 9 + e, 1) << 23);
+      for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(fabsf(feature(v[i], k))));
+      if (task < kTasks && c < sg->valid) atomicMax(col_top + c, top);
+    }
+    __syncthreads();                         // also: the parts of the segment before are written
+    Part before_this;
+    if (pending) before_this = count_part(segments + (at_segment + 2) % 3);
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const float x = v[i] * up;
-        float s = x;
+    for (int i = 0; i < kRounds; ++i) {
+      const int task = tid + i * kThreads, c = task / (NG * 4), rest = task - c * (NG * 4), gr = rest >> 2, part = rest & 3;
+      if (task < kTasks) {
+        const unsigned top = col_top[c];
+        const int e = top > 0 ? max((int)(top >> 23) - 127, -117) : 9;                     // 2^(9 - e) stays a float
+        const float up = __uint_as_float((uint32_t)(min(127 + 9 - e, 253)) << 23), down = __uint_as_float((uint32_t)max(127 - 9 + e, 1) << 23);
+        float sum = 0.f;
+        const int tl = 2 * gr + (part >> 1), hid = part & 1;                               // features 16 tl + 8 hid ..: register hid of the B operand
+        uint32_t* dst = qfrag + ((tl * NT + (c >> 3)) * 32 + (c & 7) * 4) * (kSplit ? 4 : 2) + hid;
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        // feature lane of group i: tile lane / 16, k = lane % 16; B operand of lane (c % 8, k % 8 / 2), register k / 8
-        const int tile = 2 * i + (lane >> 4), k = lane & 15;
-        const float y = k >= 8 ? x * 0.0625f : x;
-        const __half hi = __float2half_rn(y);
-        const int word = ((tile * NT + (c >> 3)) * 32 + (c & 7) * 4 + ((k & 7) >> 1)) * (kSplit ? 4 : 2) + (k >> 3);
-        __half* dst = reinterpret_cast<__half*>(qfrag + word) + (k & 1);
-        dst[0] = hi;
-        if (kSplit) dst[4] = __float2half_rn(y - __half2float(hi));
-        if (lane == 0) {
-          const __half sh = __float2half_rn(s);
-          __half* qs = reinterpret_cast<__half*>(qsum + (c >> 3) * 32 + (c & 7) * 4 + (i >> 1));
-          qs[i & 1] = sh;
-          qs[2 + (i & 1)] = __float2half_rn(s - __half2float(sh));
+        for (int k = 0; k < 4; ++k) {
+          const float x = feature(v[i], 2 * k) * up, y = feature(v[i], 2 * k + 1) * up, f = hid ? 0.0625f : 1.f;
+          sum += x + y;
+          const uint32_t h = pack(x * f, y * f);
+          dst[k * (kSplit ? 4 : 2)] = h;
+          if (kSplit) {
+            const float2 back = __half22float2(as_half2(h));
+            dst[k * 4 + 2] = pack(x * f - back.x, y * f - back.y);
+          }
         }
-      }
-      if (NG < 8 && lane < 8 && lane >= NG) {                            // groups that are not there
-        __half* qs = reinterpret_cast<__half*>(qsum + (c >> 3) * 32 + (c & 7) * 4 + (lane >> 1));
-        qs[lane & 1] = __ushort_as_half(0);
-        qs[2 + (lane & 1)] = __ushort_as_half(0);
-      }
-      if (lane == 0) {
-        const int position = sg.len - sg.T + row;
-        col_scale[c] = p.scale * (kSplit ? 1.f : 16777216.f) * down;
-        col_end[c] = c < valid ? max(0, position + 1) : 0;
-        col_from[c] = p.window > 0 ? max(0, position - p.window + 1) : 0;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (part == 0) {
+          const __half sh = __float2half_rn(sum);
+          __half* qs = reinterpret_cast<__half*>(qsum + (c >> 3) * 32 + (c & 7) * 4 + (gr >> 1));
+          qs[gr & 1] = sh;
+          qs[2 + (gr & 1)] = __float2half_rn(sum - __half2float(sh));
+          if (gr == 0) {
+            const int position = sg->position0 + (sg->tile * COLS + c) / p.G;
+            col_scale[c] = p.scale * (kSplit ? 1.f : 16777216.f) * down;
+            col_end[c] = c < sg->valid ? max(0, position + 1) : sg->highest;               // columns that are no rows have scores of 0
+            col_from[c] = c >= sg->valid ? sg->lowest : p.window > 0 ? max(0, position - p.window + 1) : 0;
+          }
+        }
       }
     }
     __syncthreads();
-    // keys that some row sees, keys that all rows see: the rows' positions ascend
-    const int lowest = col_from[0], highest = col_end[valid - 1], all_from = col_from[valid - 1], all_to = col_end[0];
+    if (pending) join_parts(segments + (at_segment + 2) % 3, before_this);
+    // the segment after this one and its first pages, to be at hand when this one's keys are through
+    const int next = at_segment == 2 ? 0 : at_segment + 1;
+    more = advance(segments + next);
+    const int page0 = more ? page_at(segments + next, 0) : -1, page1 = more ? page_at(segments + next, 1) : -1;
     float cs[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) { cs[nt][0] = col_scale[nt * 8 + 2 * t]; cs[nt][1] = col_scale[nt * 8 + 2 * t + 1]; }
 
-    // ---- ring: stage j holds this warp's two blocks of unit from_unit + j --------------------------------------------
-    const int n_stages = to_unit - from_unit;
-    const int block0 = (sg.first_unit + from_unit) * (kUnit / 16) + 2 * warp;
-    const int* row_table = p.table + (int64_t)sg.b * p.max_pages;
-    auto fetch_pages = [&](int batch) {                    // lane: block lane % 2 of stage 16 batch + lane / 2; -1: not to be read
-      const int j = batch * 16 + (lane >> 1), key = (block0 + j * (kUnit / 16) + (lane & 1)) * 16;
-      if (j >= n_stages || key >= highest || key + 16 <= lowest) return -1;
-      const int page = row_table[key >> p.shift];
-      if ((unsigned)page < (unsigned)p.n_pages) return page;
-      atomicExch(p.dev_err, kErrPage);
-      return -1;
-    };
-    int ids = fetch_pages(0), ids_next = fetch_pages(1);
-    uint32_t loaded = 0;                                   // two bits per stage of the ring
-    auto issue = [&](int j, int s) {
-      if (j > 0 && (j & 15) == 0) {
-        ids = ids_next;
-        ids_next = fetch_pages((j >> 4) + 1);
-      }
-      const int p0 = __shfl_sync(0xffffffffu, ids, (j & 15) * 2), p1 = __shfl_sync(0xffffffffu, ids, (j & 15) * 2 + 1);
-      const uint32_t bits = (p0 >= 0 ? 1u : 0u) | (p1 >= 0 ? 2u : 0u);
-      loaded = (loaded & ~(3u << (2 * s))) | bits << (2 * s);
-      if (bits && lane == 0) {
-        const int key = (block0 + j * (kUnit / 16)) * 16, inside = (key & ((1 << p.shift) - 1)) >> 4, per_page = 1 << (p.shift - 4);
-        uint8_t* dst = my_ring + s * S::kStageBytes;
-        tc::mbar_expect_tx(my_full + s, (bits == 3 ? 2 : 1) * 640 * NG);
-        if (bits == 3 && per_page > 1) {                   // neighbours in one page
-          tc::bulk_g2s(dst, p.pages + (((int64_t)p0 * p.heads + sg.head) * per_page + inside) * (640 * NG), 2 * 640 * NG, my_full + s);
-        } else {
-          if (bits & 1) tc::bulk_g2s(dst, p.pages + (((int64_t)p0 * p.heads + sg.head) * per_page + inside) * (640 * NG), 640 * NG, my_full + s);
-          if (bits & 2)
-            tc::bulk_g2s(dst + 640 * NG, p.pages + (((int64_t)p1 * p.heads + sg.head) * per_page + ((inside + 1) & (per_page - 1))) * (640 * NG), 640 * NG, my_full + s);
-        }
-      }
-    };
-    slot = 0;
-#pragma unroll
-    for (int s = 0; s < kStages; ++s)
-      if (s < n_stages) issue(s, s);
-
     // ---- one pass over the keys ----------------------------------------------------------------------------------------
+    // Weights up to 2^15 times scales above 1 may leave the halves' range.  The quick way does not look; where its sums are no numbers the segment is gone through
+    // again, scales then taken times 2^-r.
     float m[NT][2], l[NT][2], o[2 * NG][NT][4], om[NT][4];
-    int r = 0;                               // values' scales are taken times 2^-r
+    int r;
+    uint32_t seen;                           // columns that have a maximum; m of the others is 0
+    const int n_stages = sg->to_unit - sg->from_unit, first_key = (sg->first_block + 2 * warp) * 16, all_from = sg->all_from, all_to = sg->all_to;
+    for (bool careful = false;; careful = true) {
+    r = 0;
+    seen = 0;
+    bool ready = false;                      // all columns have one
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -CUDART_INF_F;
+      m[nt][0] = m[nt][1] = 0.f;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) om[nt][k] = 0.f;
@@ -323,25 +507,24 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
     }
+#pragma unroll 1
     for (int j = 0; j < n_stages; ++j) {
       const uint32_t bits = loaded >> (2 * slot) & 3u;
       if (bits) {
         tc::mbar_wait(my_full + slot, phases >> slot & 1u, dead, p.dev_err);
         phases ^= 1u << slot;
-      }
-      const int key0 = (block0 + j * (kUnit / 16)) * 16;
-      const bool whole = bits == 3u && key0 >= all_from && key0 + 32 <= all_to;
-      const uint8_t* stage = my_ring + slot * S::kStageBytes;
-      auto work = [&](auto masked_) {
-        constexpr bool kMasked = decltype(masked_)::value;
-#pragma unroll
+        const int key0 = first_key + j * kUnit;
+        // a stage that all rows see whole, once they all have a maximum, needs nothing looked at
+        const bool look = bits != 3u || key0 < all_from || key0 + 32 > all_to || !ready || careful;
+        const uint8_t* stage0 = my_ring + slot * S::kStageBytes;
+#pragma unroll 1
         for (int k0 = 0; k0 < 2; k0 += BK) {
-          if (kMasked && BK == 1 && !(bits >> k0 & 1)) continue;
+          const uint8_t* stage = stage0 + k0 * 640 * NG;
           float s[BK][NT][4];
           // minima: one MMA whose k slots are the groups, sums of q as hi (k < 8) and lo
 #pragma unroll
           for (int kb = 0; kb < BK; ++kb) {
-            const uint32_t* minima = reinterpret_cast<const uint32_t*>(stage + (k0 + kb) * 640 * NG + 544 * NG);
+            const uint32_t* minima = reinterpret_cast<const uint32_t*>(stage + kb * 640 * NG + 544 * NG);
             uint32_t x = 0, y = 0;
             if (2 * t < NG) x = minima[2 * t * 8 + g];
             if (2 * t + 1 < NG) y = minima[(2 * t + 1) * 8 + g];
@@ -349,8 +532,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const uint2 qs = qsum[nt * 32 + lane];
-              s[kb][nt][0] = s[kb][nt][1] = s[kb][nt][2] = s[kb][nt][3] = 0.f;
-              mma_half(s[kb][nt], a0, a1, a0, a1, qs.x, qs.y);
+              mma_first(s[kb][nt], a0, a1, a0, a1, qs.x, qs.y);
               if (!kSplit)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s[kb][nt][k] *= 5.9604644775390625e-8f;        // 2^-24, as the numbers
@@ -359,13 +541,9 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr) {
             float acc[BK][NT][4];
-#pragma unroll
-            for (int kb = 0; kb < BK; ++kb)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) acc[kb][nt][0] = acc[kb][nt][1] = acc[kb][nt][2] = acc[kb][nt][3] = 0.f;
             uint2 w[BK];
 #pragma unroll
-            for (int kb = 0; kb < BK; ++kb) w[kb] = *reinterpret_cast<const uint2*>(stage + (k0 + kb) * 640 * NG + gr * 256 + lane * 8);
+            for (int kb = 0; kb < BK; ++kb) w[kb] = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + gr * 256 + lane * 8);
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
               uint32_t a[BK][4];
@@ -382,17 +560,23 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                 if (kSplit) {
                   const uint4 q = *reinterpret_cast<const uint4*>(qfrag + (((2 * gr + tile) * NT + nt) * 32 + lane) * 4);
 #pragma unroll
-                  for (int kb = 0; kb < BK; ++kb) mma_split(acc[kb][nt], a[kb][0], a[kb][1], a[kb][2], a[kb][3], q.x, q.y, q.z, q.w);
+                  for (int kb = 0; kb < BK; ++kb) {
+                    if (tile) mma_split<false>(acc[kb][nt], a[kb][0], a[kb][1], a[kb][2], a[kb][3], q.x, q.y, q.z, q.w);
+                    else mma_split<true>(acc[kb][nt], a[kb][0], a[kb][1], a[kb][2], a[kb][3], q.x, q.y, q.z, q.w);
+                  }
                 } else {
                   const uint2 q = *reinterpret_cast<const uint2*>(qfrag + (((2 * gr + tile) * NT + nt) * 32 + lane) * 2);
 #pragma unroll
-                  for (int kb = 0; kb < BK; ++kb) mma_half(acc[kb][nt], a[kb][0], a[kb][1], a[kb][2], a[kb][3], q.x, q.y);
+                  for (int kb = 0; kb < BK; ++kb) {
+                    if (tile) mma_half(acc[kb][nt], a[kb][0], a[kb][1], a[kb][2], a[kb][3], q.x, q.y);
+                    else mma_first(acc[kb][nt], a[kb][0], a[kb][1], a[kb][2], a[kb][3], q.x, q.y);
+                  }
                 }
               }
             }
 #pragma unroll
             for (int kb = 0; kb < BK; ++kb) {
-              const float2 sc = __half22float2(as_half2(reinterpret_cast<const uint32_t*>(stage + (k0 + kb) * 640 * NG + 512 * NG)[gr * 8 + g]));
+              const float2 sc = __half22float2(as_half2(reinterpret_cast<const uint32_t*>(stage + kb * 640 * NG + 512 * NG)[gr * 8 + g]));
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 s[kb][nt][0] = fmaf(sc.x, acc[kb][nt][0], s[kb][nt][0]);
@@ -402,122 +586,135 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
               }
             }
           }
-          // scores in units of log2; the maximum is raised only when it lags by more than 2^8, so most blocks need no exchange between lanes
-          float top[NT][2];
+          // values' scales and minima (rows = groups), in the order of the weights' operand
+          uint2 vs[BK][NG], mn[BK];
+#pragma unroll
+          for (int kb = 0; kb < BK; ++kb) {
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) vs[kb][gr] = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 576 * NG + gr * 32 + t * 8);
+            mn[kb] = make_uint2(0, 0);
+            if (g < NG) mn[kb] = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 608 * NG + g * 32 + t * 8);
+          }
+          // scores in units of log2, less the maximum as far as it is known, plus 7: weights are 2^7 p.  The maximum is raised only when it lags by more than 2^8, so most
+          // blocks need no exchange between lanes.
           bool raise = false;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int kb = 0; kb < BK; ++kb)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                s[kb][nt][k] *= cs[nt][k & 1];
-                if (kMasked) {
-                  const int key = key0 + (k0 + kb) * 16 + g + (k >= 2 ? 8 : 0), c = nt * 8 + 2 * t + (k & 1);
-                  if (key >= col_end[c] || key < col_from[c] || !(bits >> (k0 + kb) & 1)) s[kb][nt][k] = -CUDART_INF_F;
-                }
-              }
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              top[nt][k] = fmaxf(s[0][nt][k], s[0][nt][k + 2]);
-              if (BK == 2) top[nt][k] = fmaxf(top[nt][k], fmaxf(s[BK - 1][nt][k], s[BK - 1][nt][k + 2]));
-              raise |= top[nt][k] > m[nt][k] + 8.f;
-            }
-          }
-          // values' scales, in the order of the weights' operand
-          uint2 vs[BK][NG];
-          __half2 most = __float2half2_rn(0.f);
+              float top = -CUDART_INF_F;
+              const float less = kPScale - m[nt][k];
 #pragma unroll
-          for (int kb = 0; kb < BK; ++kb)
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-              vs[kb][gr] = *reinterpret_cast<const uint2*>(stage + (k0 + kb) * 640 * NG + 576 * NG + gr * 32 + t * 8);
-              if (kMasked && !(bits >> (k0 + kb) & 1)) vs[kb][gr] = make_uint2(0, 0);
-              most = __hmax2(most, __hmax2(as_half2(vs[kb][gr].x), as_half2(vs[kb][gr].y)));
+              for (int kb = 0; kb < BK; ++kb) {
+                s[kb][nt][k] = fmaf(s[kb][nt][k], cs[nt][k], less);
+                s[kb][nt][k + 2] = fmaf(s[kb][nt][k + 2], cs[nt][k], less);
+                top = fmaxf(top, fmaxf(s[kb][nt][k], s[kb][nt][k + 2]));
+              }
+              raise |= top > kPScale + 8.f;
             }
-          const float most_s = fmaxf(__low2float(most), __high2float(most));
-          const float limit = __uint_as_float((uint32_t)(127 + r) << 23);                  // 2^r: weights up to 2^15 times scales up to 1 stay halves
-          if (__any_sync(0xffffffffu, raise || most_s > limit)) {
+          if (look || __any_sync(0xffffffffu, raise)) {
+            if (look) {
+              __half2 most = __float2half2_rn(0.f);
+#pragma unroll
+              for (int kb = 0; kb < BK; ++kb) {
+                const bool there = bits >> (k0 + kb) & 1;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const int key = key0 + (k0 + kb) * 16 + g + (k >= 2 ? 8 : 0), c = nt * 8 + 2 * t + (k & 1);
+                    if (key >= col_end[c] || key < col_from[c] || !there) s[kb][nt][k] = -CUDART_INF_F;
+                  }
+                // A key's value that is no number counts for the rows that see the key alone: a minimum that is none makes its scale one, and scales meet weights below.
+                // A key that no row sees counts for none.
+                if (!there) mn[kb] = make_uint2(0, 0);
+                const uint32_t ox = __vcmpgtu2(mn[kb].x & 0x7fff7fffu, 0x7bff7bffu), oy = __vcmpgtu2(mn[kb].y & 0x7fff7fffu, 0x7bff7bffu);
+                mn[kb].x &= ~ox;
+                mn[kb].y &= ~oy;
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) {
+                  if (!there) vs[kb][gr] = make_uint2(0, 0);
+                  most = __hmax2(most, __hmax2(as_half2(vs[kb][gr].x), as_half2(vs[kb][gr].y)));
+                  vs[kb][gr].x |= __shfl_sync(0xffffffffu, ox, gr * 4 + t) & 0x7fff7fffu;
+                  vs[kb][gr].y |= __shfl_sync(0xffffffffu, oy, gr * 4 + t) & 0x7fff7fffu;
+                }
+              }
+              float x = fmaxf(__low2float(most), __high2float(most));
+#pragma unroll
+              for (int off = 1; off < 4; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+              if (x > __uint_as_float((uint32_t)(127 + r) << 23) && x <= 65504.f) {        // above 2^r: weights up to 2^15 times scales up to 1 stay halves
+                const int rn = (int)(__float_as_uint(x) >> 23) - 126;                      // x < 2^rn
+                const float fade = __uint_as_float((uint32_t)(127 + r - rn) << 23);
+                r = rn;
+#pragma unroll
+                for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[i][nt][k] *= fade;
+              }
+              if (r) {
+                const __half2 down = __float2half2_rn(__uint_as_float((uint32_t)(127 - r) << 23));
+#pragma unroll
+                for (int kb = 0; kb < BK; ++kb)
+#pragma unroll
+                  for (int gr = 0; gr < NG; ++gr) {
+                    vs[kb][gr].x = as_u32(__hmul2(as_half2(vs[kb][gr].x), down));
+                    vs[kb][gr].y = as_u32(__hmul2(as_half2(vs[kb][gr].y), down));
+                  }
+              }
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                float x = top[nt][k];
+                float x = fmaxf(s[0][nt][k], s[0][nt][k + 2]);
+                if (BK == 2) x = fmaxf(x, fmaxf(s[BK - 1][nt][k], s[BK - 1][nt][k + 2]));
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                if (x > m[nt][k]) {
-                  const float fade = exp2f(m[nt][k] - x);
-                  m[nt][k] = x;
+                const float rise = x - kPScale;
+                const bool first = !(seen >> (2 * nt + k) & 1);
+                if (first ? x > -CUDART_INF_F : rise > 0.f) {
+                  const float fade = first ? 0.f : exp2_fast(-rise);
+                  seen |= 1u << (2 * nt + k);
+                  m[nt][k] += rise;
                   l[nt][k] *= fade;
                   om[nt][k] *= fade;
                   om[nt][k + 2] *= fade;
 #pragma unroll
                   for (int i = 0; i < 2 * NG; ++i) { o[i][nt][k] *= fade; o[i][nt][k + 2] *= fade; }
+#pragma unroll
+                  for (int kb = 0; kb < BK; ++kb) { s[kb][nt][k] -= rise; s[kb][nt][k + 2] -= rise; }
                 }
               }
-            float x = most_s;
-#pragma unroll
-            for (int off = 1; off < 4; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-            if (x > limit && x <= 65504.f) {
-              const int rn = (int)(__float_as_uint(x) >> 23) - 126;                        // x < 2^rn
-              const float fade = __uint_as_float((uint32_t)(127 + r - rn) << 23);
-              r = rn;
-#pragma unroll
-              for (int i = 0; i < 2 * NG; ++i)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) o[i][nt][k] *= fade;
-            }
+            // (larger scales keep the quick way closed)
+            ready = r == 0 && __all_sync(0xffffffffu, seen == (1u << (2 * NT)) - 1u);
           }
-          // weights: 2^7 exp2(score - m) as halves (float32: two of them), from accumulators to B operands
-          uint32_t pb[BK][NT][kSplit ? 4 : 2];
+          // weights as halves (float32: two of them), from accumulators to B operands; then values
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float m0 = (m[nt][0] == -CUDART_INF_F ? 0.f : m[nt][0]) - kPScale, m1 = (m[nt][1] == -CUDART_INF_F ? 0.f : m[nt][1]) - kPScale;
+          for (int kb = 0; kb < BK; ++kb) {
+            uint32_t pb[NT][kSplit ? 4 : 2];
 #pragma unroll
-            for (int kb = 0; kb < BK; ++kb) {
+            for (int nt = 0; nt < NT; ++nt) {
               float e[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) e[k] = exp2f(s[kb][nt][k] - (k & 1 ? m1 : m0));
+              for (int k = 0; k < 4; ++k) e[k] = exp2_fast(s[kb][nt][k]);
               l[nt][0] += e[0] + e[2];
               l[nt][1] += e[1] + e[3];
               const uint32_t h0 = pack(e[0], e[1]), h1 = pack(e[2], e[3]);
-              pb[kb][nt][0] = transposed(h0);
-              pb[kb][nt][1] = transposed(h1);
+              pb[nt][0] = transposed(h0);
+              pb[nt][1] = transposed(h1);
               if (kSplit) {
                 const float2 f0 = __half22float2(as_half2(h0)), f1 = __half22float2(as_half2(h1));
-                pb[kb][nt][kSplit ? 2 : 0] = transposed(pack(e[0] - f0.x, e[1] - f0.y));
-                pb[kb][nt][kSplit ? 3 : 0] = transposed(pack(e[2] - f1.x, e[3] - f1.y));
+                pb[nt][kSplit ? 2 : 0] = transposed(pack(e[0] - f0.x, e[1] - f0.y));
+                pb[nt][kSplit ? 3 : 0] = transposed(pack(e[2] - f1.x, e[3] - f1.y));
               }
+              if (kSplit) mma_split<false>(om[nt], mn[kb].x, 0u, mn[kb].y, 0u, pb[nt][0], pb[nt][1], pb[nt][kSplit ? 2 : 0], pb[nt][kSplit ? 3 : 0]);
+              else mma_half(om[nt], mn[kb].x, 0u, mn[kb].y, 0u, pb[nt][0], pb[nt][1]);
             }
-          }
-          // values: minima (rows = groups), then numbers times scales
-#pragma unroll
-          for (int kb = 0; kb < BK; ++kb) {
-            uint2 mn = make_uint2(0, 0);
-            if (g < NG) mn = *reinterpret_cast<const uint2*>(stage + (k0 + kb) * 640 * NG + 608 * NG + g * 32 + t * 8);
-            if (kMasked) {
-              // a key without a page has no minima; a minimum that is no number counts through its scale, and so only for the rows that see its key
-              if (!(bits >> (k0 + kb) & 1)) mn = make_uint2(0, 0);
-              const uint32_t ox = __vcmpgtu2(mn.x & 0x7fff7fffu, 0x7bff7bffu), oy = __vcmpgtu2(mn.y & 0x7fff7fffu, 0x7bff7bffu);
-              mn.x &= ~ox;
-              mn.y &= ~oy;
-#pragma unroll
-              for (int gr = 0; gr < NG; ++gr) {
-                vs[kb][gr].x |= __shfl_sync(0xffffffffu, ox, gr * 4 + t) & 0x7fff7fffu;
-                vs[kb][gr].y |= __shfl_sync(0xffffffffu, oy, gr * 4 + t) & 0x7fff7fffu;
-              }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (kSplit) mma_split(om[nt], mn.x, 0u, mn.y, 0u, pb[kb][nt][0], pb[kb][nt][1], pb[kb][nt][kSplit ? 2 : 0], pb[kb][nt][kSplit ? 3 : 0]);
-              else mma_half(om[nt], mn.x, 0u, mn.y, 0u, pb[kb][nt][0], pb[kb][nt][1]);
-            }
-            const float down_r = __uint_as_float((uint32_t)(127 - r) << 23);
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-              const uint2 w = *reinterpret_cast<const uint2*>(stage + (k0 + kb) * 640 * NG + 256 * NG + gr * 256 + lane * 8);
+              const uint2 w = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 256 * NG + gr * 256 + lane * 8);
               uint32_t wb[NT][kSplit ? 4 : 2];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
@@ -525,10 +722,9 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                   const float2 sx = __half22float2(as_half2(vs[kb][gr].x)), sy = __half22float2(as_half2(vs[kb][gr].y));
 #pragma unroll
                   for (int i = 0; i < 2; ++i) {
-                    const float2 hi = __half22float2(as_half2(pb[kb][nt][i])), lo = __half22float2(as_half2(pb[kb][nt][kSplit ? 2 + i : 0]));
-                    const float2 sc = i ? sy : sx;
-                    float x = (hi.x + lo.x) * (sc.x * down_r), y = (hi.y + lo.y) * (sc.y * down_r);
-                    if (kMasked) {
+                    const float2 hi = __half22float2(as_half2(pb[nt][i])), lo = __half22float2(as_half2(pb[nt][kSplit ? 2 + i : 0]));
+                    float x = (hi.x + lo.x) * (i ? sy.x : sx.x), y = (hi.y + lo.y) * (i ? sy.y : sx.y);
+                    if (look) {
                       if (hi.x == 0.f) x = 0.f;
                       if (hi.y == 0.f) y = 0.f;
                     }
@@ -537,18 +733,15 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                     wb[nt][kSplit ? 2 + i : 0] = pack(x - f.x, y - f.y);
                   }
                 } else {
-                  __half2 sx = as_half2(vs[kb][gr].x), sy = as_half2(vs[kb][gr].y);
-                  if (r) {
-                    const __half2 dr = __float2half2_rn(down_r);
-                    sx = __hmul2(sx, dr);
-                    sy = __hmul2(sy, dr);
-                  }
-                  wb[nt][0] = as_u32(__hmul2(as_half2(pb[kb][nt][0]), sx));
-                  wb[nt][1] = as_u32(__hmul2(as_half2(pb[kb][nt][1]), sy));
-                  if (kMasked) {
-                    wb[nt][0] &= __vcmpne2(pb[kb][nt][0] & 0x7fff7fffu, 0u);
-                    wb[nt][1] &= __vcmpne2(pb[kb][nt][1] & 0x7fff7fffu, 0u);
-                  }
+                  wb[nt][0] = as_u32(__hmul2(as_half2(pb[nt][0]), as_half2(vs[kb][gr].x)));
+                  wb[nt][1] = as_u32(__hmul2(as_half2(pb[nt][1]), as_half2(vs[kb][gr].y)));
+                }
+              }
+              if (!kSplit && look) {         // a weight of 0 takes no part
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  wb[nt][0] &= __vcmpne2(pb[nt][0], 0u);
+                  wb[nt][1] &= __vcmpne2(pb[nt][1], 0u);
                 }
               }
 #pragma unroll
@@ -558,22 +751,41 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                                a3 = numbers<kSplit>(x >> 8, 0x00f000f0u);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                  if (kSplit) mma_split(o[2 * gr + tile][nt], a0, a1, a2, a3, wb[nt][0], wb[nt][1], wb[nt][kSplit ? 2 : 0], wb[nt][kSplit ? 3 : 0]);
+                  if (kSplit) mma_split<false>(o[2 * gr + tile][nt], a0, a1, a2, a3, wb[nt][0], wb[nt][1], wb[nt][kSplit ? 2 : 0], wb[nt][kSplit ? 3 : 0]);
                   else mma_half(o[2 * gr + tile][nt], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
                 }
               }
             }
           }
         }
-      };
-      if (whole) work(std::false_type());
-      else if (bits) work(std::true_type());
+      }
       __syncwarp();
-      if (j + kStages < n_stages) issue(j + kStages, slot);
+      if (j + kStages < n_stages) issue(sg, j + kStages, slot);
       slot = slot + 1 == kStages ? 0 : slot + 1;
     }
 
-    // ---- the warps' sums become one ------------------------------------------------------------------------------------
+    float all = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) all = fmaf(o[i][nt][k], 0.f, all);
+      }
+    if (careful || !__any_sync(0xffffffffu, all != 0.f)) break;          // NaN is not 0 either
+    start(sg, page_at(sg, 0), page_at(sg, 1));
+    }
+
+    // ---- the next segment's keys are asked for while this one's sums become one -------------------------------------------------
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (!(seen >> (2 * nt + k) & 1)) m[nt][k] = -CUDART_INF_F;
+    if (more) {
+      start(segments + next, page0, page1);
+      load_queries(segments + next, v);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -585,7 +797,8 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
           warp_l[warp * COLS + nt * 8 + 2 * t + k] = l[nt][k];
         }
       }
-    __syncthreads();                         // all warps are through with the ring
+    __syncthreads();
+    if (tid < COLS) col_top[tid] = 0;
     float fade[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -594,89 +807,59 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
         float top = -CUDART_INF_F;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + k]);
-        fade[nt][k] = m[nt][k] == -CUDART_INF_F ? (l[nt][k] != l[nt][k] ? 1.f : 0.f) : exp2f(m[nt][k] - top);
+        fade[nt][k] = m[nt][k] == -CUDART_INF_F ? (l[nt][k] != l[nt][k] ? 1.f : 0.f) : exp2_fast(m[nt][k] - top);
       }
     const float up_r = __uint_as_float((uint32_t)(127 + (kSplit ? -4 : 20) + r) << 23);  // of 16 n; n takes another 16
 #pragma unroll
-    for (int i = 0; i < 2 * NG; ++i)
+    for (int turn = 0; turn < 2; ++turn) {   // warps 0 and 1 write, 2 and 3 add
+      if (warp >> 1 == turn) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float b0 = __shfl_sync(0xffffffffu, om[nt][0], (i >> 1) * 4 + t), b1 = __shfl_sync(0xffffffffu, om[nt][1], (i >> 1) * 4 + t);
-        float* dst = merge + (warp * COLS + nt * 8 + 2 * t) * S::kPitch + 16 * i + g;
-        dst[0] = fmaf(o[i][nt][0], up_r * 16.f, b0) * fade[nt][0];
-        dst[S::kPitch] = fmaf(o[i][nt][1], up_r * 16.f, b1) * fade[nt][1];
-        dst[8] = fmaf(o[i][nt][2], up_r, b0) * fade[nt][0];
-        dst[S::kPitch + 8] = fmaf(o[i][nt][3], up_r, b1) * fade[nt][1];
+        for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float b0 = __shfl_sync(0xffffffffu, om[nt][0], (i >> 1) * 4 + t), b1 = __shfl_sync(0xffffffffu, om[nt][1], (i >> 1) * 4 + t);
+            float* dst = merge + ((warp & 1) * COLS + nt * 8 + 2 * t) * S::kPitch + 16 * i + g;
+            const float x0 = fmaf(o[i][nt][0], up_r * 16.f, b0) * fade[nt][0], x1 = fmaf(o[i][nt][1], up_r * 16.f, b1) * fade[nt][1];
+            const float x2 = fmaf(o[i][nt][2], up_r, b0) * fade[nt][0], x3 = fmaf(o[i][nt][3], up_r, b1) * fade[nt][1];
+            if (turn == 0) {
+              dst[0] = x0; dst[S::kPitch] = x1; dst[8] = x2; dst[S::kPitch + 8] = x3;
+            } else {
+              dst[0] += x0; dst[S::kPitch] += x1; dst[8] += x2; dst[S::kPitch + 8] += x3;
+            }
+          }
       }
-    __syncthreads();
-    const bool alone = from_unit == 0 && to_unit == sg.n_units;
-    const int part = (int)blockIdx.x * 2 + (from_unit == 0 ? 1 : 0);
-    auto put = [&](int c, int d, float4 v, float L) {
-      const float inv = L > 0.f || L != L ? 1.f / L : 0.f;             // a row that sees no key is 0
-      const int rho = sg.tile * COLS + c, row = rho / p.G, hq = rho - row * p.G;
-      T* out = reinterpret_cast<T*>(p.out) + (int64_t)(sg.rows0 + row) * p.out_stride + (int64_t)(sg.head * p.G + hq) * D + d;
-      if (kSplit) {
-        *reinterpret_cast<float4*>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      } else {
-        __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv), y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-        *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
-      }
-    };
-    for (int i = tid; i < valid * (D / 4); i += kThreads) {
+      __syncthreads();
+    }
+    const bool alone = sg->from_unit == 0 && sg->to_unit == sg->n_units;
+    const int part = (int)blockIdx.x * 2 + (sg->from_unit == 0 ? 1 : 0);
+    for (int i = tid; i < sg->valid * (D / 4); i += kThreads) {
       const int c = i / (D / 4), d = (i - c * (D / 4)) * 4;
       float top = -CUDART_INF_F, L = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + c]);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float mw = warp_m[w * COLS + c], lw = warp_l[w * COLS + c];
-        L += mw == -CUDART_INF_F ? (lw != lw ? lw : 0.f) : lw * exp2f(mw - top);
-        const float4 x = *reinterpret_cast<const float4*>(merge + (w * COLS + c) * S::kPitch + d);
-        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        L += mw == -CUDART_INF_F ? (lw != lw ? lw : 0.f) : lw * exp2_fast(mw - top);
       }
+      const float4 x = *reinterpret_cast<const float4*>(merge + c * S::kPitch + d), y = *reinterpret_cast<const float4*>(merge + (COLS + c) * S::kPitch + d);
+      const float4 w = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
       if (alone) {
-        put(c, d, v, L);
+        put(sg, c, d, w, L);
       } else {
-        __stcg(reinterpret_cast<float4*>(p.part_o + ((int64_t)part * COLS + c) * D + d), v);
+        __stcg(reinterpret_cast<float4*>(p.part_o + ((int64_t)part * COLS + c) * D + d), w);
         if (d == 0) __stcg(p.part_ml + part * COLS + c, make_float2(top, L));
       }
     }
-    if (!alone) {
-      // the last of the CTAs that share the triple joins what all of them left
-      const int64_t last_unit = sg.item0 + sg.n_units - 1;
-      const int ca = (int)(((sg.item0 + 1) * grid - 1) / U), cb = (int)(((last_unit + 1) * grid - 1) / U), n = cb - ca + 1;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const bool last = atomicAdd(p.counters + ca, 1u) == (unsigned)n - 1u;
-        if (last) p.counters[ca] = 0u;
-        shared_word[0] = last;
-      }
-      __syncthreads();
-      if (shared_word[0]) {
-        __threadfence();
-        for (int i = tid; i < valid * (D / 4); i += kThreads) {
-          const int c = i / (D / 4), d = (i - c * (D / 4)) * 4;
-          float top = -CUDART_INF_F;
-#pragma unroll 8
-          for (int k = 0; k < n; ++k) top = fmaxf(top, __ldcg(&p.part_ml[((ca + k) * 2 + (k == 0)) * COLS + c].x));
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          float L = 0.f;
-#pragma unroll 8
-          for (int k = 0; k < n; ++k) {
-            const int64_t from = (int64_t)((ca + k) * 2 + (k == 0)) * COLS + c;
-            const float2 ml = __ldcg(p.part_ml + from);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + from * D + d));
-            const float f = ml.x == -CUDART_INF_F ? (ml.y != ml.y ? 1.f : 0.f) : exp2f(ml.x - top);
-            L = fmaf(ml.y, f, L);
-            v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
-          }
-          put(c, d, v, L);
-        }
-      }
-    }
-    tc::fence_async_smem();                  // the next segment's copies overwrite what was joined here
+    pending = !alone;
+    if (!more) break;
+    at_segment = next;
+  }
+  if (pending) {
+    __syncthreads();
+    const Part last = count_part(segments + at_segment);
+    __syncthreads();
+    join_parts(segments + at_segment, last);
   }
 }
 
@@ -684,9 +867,9 @@ template <typename T, int NG, int NT> int32_t configure_one(Variant* v) {
   using S = Shape<T, NG, NT>;
   v->kernel = attention_kernel<T, NG, NT>;
   v->smem = S::kFixed;
-  const int most = S::kFixed + (kMaxSeqs + 1) * 4;
+  const int most = S::kFixed + seq_bytes(kMaxSeqs);
   LMB_CUDA(cudaFuncSetAttribute(v->kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-  LMB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v->ctas_per_sm, v->kernel, kThreads, (size_t)S::kFixed + 260 * 4));
+  LMB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v->ctas_per_sm, v->kernel, kThreads, (size_t)S::kFixed + seq_bytes(64)));
   return LMB200_OK;
 }
 
