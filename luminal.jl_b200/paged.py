@@ -7,87 +7,121 @@ legacy default stream)."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 from . import _lib
 from ._lib import BF16, F32, I32
 from .device import DeviceArray
 
-_TORCH = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.int32": I32}
+_functions = {}
 
 
-def _float(what, a):
-    """(address, dtype code) of a float32 or bfloat16 array."""
-    code = a.dtype if isinstance(a, DeviceArray) else _TORCH.get(str(a.dtype))
-    if code not in (F32, BF16):
-        raise ValueError(f"{what}: {a.dtype}, expected float32 or bfloat16")
-    return _address(what, a), code
+def _call(name, *args):
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(_lib.load(), name)
+    status = f(*args)
+    if status:
+        _lib.check(status)
+
+
+_NAMES = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.int32": I32}
+_CODES = {F32: F32, BF16: BF16, I32: I32}     # dtype, of a DeviceArray or as torch spells it -> code
+
+
+def _code(a):
+    try:
+        return _CODES[a.dtype]
+    except KeyError:
+        return _CODES.setdefault(a.dtype, _NAMES.get(str(a.dtype), -1))
+
+
+def _count(a):
+    try:
+        return a.numel()
+    except AttributeError:
+        return math.prod(a.shape)
 
 
 def _address(what, a):
     if isinstance(a, DeviceArray):
         return a.ptr
-    if not getattr(a, "is_cuda", True):
+    if not a.is_cuda:
         raise ValueError(f"{what}: not in device memory")
     return a.data_ptr()
 
 
-def _ints(what, a, least):
-    """Address of a contiguous int32 array of at least `least` elements."""
-    if (a.dtype if isinstance(a, DeviceArray) else _TORCH.get(str(a.dtype))) != I32:
-        raise ValueError(f"{what}: {a.dtype}, expected int32")
-    return _plain(what, a, least)
-
-
 def _plain(what, a, least):
-    n = 1
-    for d in a.shape:
-        n *= d
-    if n < least:
-        raise ValueError(f"{what}: {n} elements, at least {least} are needed")
+    """Address of a contiguous array of at least `least` elements."""
+    if _count(a) < least:
+        raise ValueError(f"{what}: {_count(a)} elements, at least {least} are needed")
     if not isinstance(a, DeviceArray) and not a.is_contiguous():
         raise ValueError(f"{what}: not contiguous")
     return _address(what, a)
 
 
+def _ints(what, a, least):
+    try:                                       # a step names a dozen of these: torch's own answers first
+        if _CODES[a.dtype] == I32 and a.numel() >= least and a.is_cuda and a.is_contiguous():
+            return a.data_ptr()
+    except (KeyError, AttributeError):
+        pass
+    if _code(a) != I32:
+        raise ValueError(f"{what}: {a.dtype}, expected int32")
+    return _plain(what, a, least)
+
+
+def _float(what, a):
+    """(address, dtype code) of a float32 or bfloat16 array."""
+    code = _code(a)
+    if code != F32 and code != BF16:
+        raise ValueError(f"{what}: {a.dtype}, expected float32 or bfloat16")
+    return _address(what, a), code
+
+
 def _rows(what, a, inner):
     """Row pitch in elements of an array [rows, ...] whose rows are contiguous and `inner` long."""
-    n = 1
-    for d in a.shape[1:]:
-        n *= d
-    if n != inner:
-        raise ValueError(f"{what}: rows of {n} elements, expected {inner}")
-    if isinstance(a, DeviceArray):
+    rows = a.shape[0]
+    if _count(a) != rows * inner:
+        raise ValueError(f"{what}: {_count(a)} elements for {rows} rows of {inner}")
+    if isinstance(a, DeviceArray) or a.is_contiguous():
         return inner
-    step = 1
-    for d, s in zip(reversed(a.shape[1:]), reversed(a.stride()[1:])):
-        if d > 1 and s != step:
+    step, strides = 1, a.stride()
+    for i in range(len(strides) - 1, 0, -1):
+        if a.shape[i] > 1 and strides[i] != step:
             raise ValueError(f"{what}: the elements of a row must be contiguous")
-        step *= d
-    return a.stride(0) if a.shape[0] > 1 else inner
+        step *= a.shape[i]
+    return strides[0] if rows > 1 else inner
 
 
 def kv4_page_bytes(page_size, n_kv_heads, head_dim):
     """Bytes of one page of one layer's cache."""
     n = C.c_int64(0)
-    _lib.call("lmb200_kv4_page_bytes", int(page_size), int(n_kv_heads), int(head_dim), C.byref(n))
+    _call("lmb200_kv4_page_bytes", int(page_size), int(n_kv_heads), int(head_dim), C.byref(n))
     return n.value
 
 
+_PAGE_BYTES = {}
+
+
+def _bytes(a):
+    return _count(a) * ((2 if a.dtype == BF16 else 4) if isinstance(a, DeviceArray) else a.element_size())
+
+
 def _pool(pages, page_size, heads, dim):
-    n_pages = pages.shape[0]
-    size = 1
-    for d in pages.shape:
-        size *= d
-    each = 4 if isinstance(pages, DeviceArray) and pages.dtype != BF16 else 2 if isinstance(pages, DeviceArray) else pages.element_size()
-    if size * each < n_pages * kv4_page_bytes(page_size, heads, dim):
-        raise ValueError(f"pages: {size * each} bytes for {n_pages} pages of {kv4_page_bytes(page_size, heads, dim)}")
+    n_pages, shape = pages.shape[0], (page_size, heads, dim)
+    each = _PAGE_BYTES.get(shape)
+    if each is None:
+        each = _PAGE_BYTES[shape] = kv4_page_bytes(*shape)
+    if _bytes(pages) < n_pages * each:
+        raise ValueError(f"pages: {_bytes(pages)} bytes for {n_pages} pages of {each}")
     return _plain("pages", pages, 0), n_pages
 
 
 def kv_reserve(device, lens, add, table, free_list, n_free, *, page_size, lens_out, n_free_out, cu_rows, slots, status):
     """Pages, slots and lengths for add[b] more tokens of every sequence (lmb200_kv_reserve).  lens_out may be lens, n_free_out n_free."""
     n, rows = lens.shape[0], slots.shape[0]
-    _lib.call("lmb200_kv_reserve", device.handle, n, page_size, table.shape[1], free_list.shape[0], rows, _ints("lens", lens, n), _ints("add", add, n),
+    _call("lmb200_kv_reserve", device.handle, n, page_size, table.shape[1], free_list.shape[0], rows, _ints("lens", lens, n), _ints("add", add, n),
               _ints("table", table, n * table.shape[1]), _ints("free_list", free_list, 1), _ints("n_free", n_free, 1), _ints("lens_out", lens_out, n),
               _ints("n_free_out", n_free_out, 1), _ints("cu_rows", cu_rows, n + 1), _ints("slots", slots, 0), _ints("status", status, 1))
 
@@ -95,7 +129,7 @@ def kv_reserve(device, lens, add, table, free_list, n_free, *, page_size, lens_o
 def kv_shrink(device, lens, drop, table, free_list, n_free, *, page_size, lens_out, n_free_out):
     """The last drop[b] tokens of every sequence leave the cache and their pages go back (lmb200_kv_shrink)."""
     n = lens.shape[0]
-    _lib.call("lmb200_kv_shrink", device.handle, n, page_size, table.shape[1], free_list.shape[0], _ints("lens", lens, n), _ints("drop", drop, n),
+    _call("lmb200_kv_shrink", device.handle, n, page_size, table.shape[1], free_list.shape[0], _ints("lens", lens, n), _ints("drop", drop, n),
               _ints("table", table, n * table.shape[1]), _ints("free_list", free_list, 1), _ints("n_free", n_free, 1), _ints("lens_out", lens_out, n),
               _ints("n_free_out", n_free_out, 1))
 
@@ -103,10 +137,10 @@ def kv_shrink(device, lens, drop, table, free_list, n_free, *, page_size, lens_o
 def _store(name, device, k, v, slots, pages, page_size):
     rows, heads, dim = k.shape
     (kp, code), (vp, v_code) = _float("k", k), _float("v", v)
-    if code != v_code or tuple(v.shape) != tuple(k.shape):
+    if code != v_code or v.shape != k.shape:
         raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
     pool, n_pages = _pool(pages, page_size, heads, dim)
-    _lib.call(name, device.handle, code, kp, vp, _rows("k", k, heads * dim), _rows("v", v, heads * dim), rows, heads, dim, _ints("slots", slots, rows), pool, n_pages,
+    _call(name, device.handle, code, kp, vp, _rows("k", k, heads * dim), _rows("v", v, heads * dim), rows, heads, dim, _ints("slots", slots, rows), pool, n_pages,
               page_size)
 
 
@@ -123,15 +157,8 @@ def kv4_read(device, k_out, v_out, slots, pages, *, page_size):
 def kv4_attention_workspace(device, head_dim):
     """Bytes of workspace that kv4_attention takes; zero before the first call."""
     n = C.c_int64(0)
-    _lib.call("lmb200_kv4_attention_workspace", device.handle, int(head_dim), C.byref(n))
+    _call("lmb200_kv4_attention_workspace", device.handle, int(head_dim), C.byref(n))
     return n.value
-
-
-def _bytes(a):
-    n = 1
-    for d in a.shape:
-        n *= d
-    return n * ((2 if a.dtype == BF16 else 4) if isinstance(a, DeviceArray) else a.element_size())
 
 
 def kv4_attention(device, q, out, cu_rows, lens, table, pages, *, page_size, workspace, scale=None, window=0):
@@ -139,13 +166,13 @@ def kv4_attention(device, q, out, cu_rows, lens, table, pages, *, page_size, wor
     rows, n_heads, dim = q.shape
     n = lens.shape[0]
     (qp, code), (op, out_code) = _float("q", q), _float("out", out)
-    if code != out_code or tuple(out.shape) != tuple(q.shape):
+    if code != out_code or out.shape != q.shape:
         raise ValueError(f"q {q.dtype} {tuple(q.shape)} and out {out.dtype} {tuple(out.shape)} differ")
     heads = pages.shape[1]
     if n_heads % heads:
         raise ValueError(f"{n_heads} query heads over {heads} kv heads")
     pool, n_pages = _pool(pages, page_size, heads, dim)
-    _lib.call("lmb200_kv4_attention", device.handle, code, qp, _rows("q", q, n_heads * dim), op, _rows("out", out, n_heads * dim), rows, n, _ints("cu_rows", cu_rows, n + 1),
+    _call("lmb200_kv4_attention", device.handle, code, qp, _rows("q", q, n_heads * dim), op, _rows("out", out, n_heads * dim), rows, n, _ints("cu_rows", cu_rows, n + 1),
               _ints("lens", lens, n), _ints("table", table, n * table.shape[1]), table.shape[1], pool, n_pages, page_size, heads, n_heads // heads, dim,
               dim ** -0.5 if scale is None else scale, window, _address("workspace", workspace), _bytes(workspace))
 
@@ -153,7 +180,7 @@ def kv4_attention(device, q, out, cu_rows, lens, table, pages, *, page_size, wor
 def verify_drafts_workspace(rows):
     """Bytes of workspace that verify_drafts takes for so many rows."""
     n = C.c_int64(0)
-    _lib.call("lmb200_verify_drafts_workspace", int(rows), C.byref(n))
+    _call("lmb200_verify_drafts_workspace", int(rows), C.byref(n))
     return n.value
 
 
@@ -166,7 +193,7 @@ def verify_drafts(device, target, draft, cu_rows, tokens, temperature, accept_u,
     dp, d_stride = None, 0
     if draft is not None:
         dp, d_code = _float("draft", draft)
-        if d_code != code or tuple(draft.shape) != tuple(target.shape):
+        if d_code != code or draft.shape != target.shape:
             raise ValueError(f"target {target.dtype} {tuple(target.shape)} and draft {draft.dtype} {tuple(draft.shape)} differ")
         d_stride = _rows("draft", draft, vocab)
     randoms = []
@@ -177,7 +204,7 @@ def verify_drafts(device, target, draft, cu_rows, tokens, temperature, accept_u,
         if _float(what, a)[1] != F32:
             raise ValueError(f"{what}: {a.dtype}, expected float32")
         randoms.append(_plain(what, a, least))
-    _lib.call("lmb200_verify_drafts", device.handle, code, tp, _rows("target", target, vocab), dp, d_stride, vocab, rows, n, _ints("cu_rows", cu_rows, n + 1),
+    _call("lmb200_verify_drafts", device.handle, code, tp, _rows("target", target, vocab), dp, d_stride, vocab, rows, n, _ints("cu_rows", cu_rows, n + 1),
               _ints("tokens", tokens, rows), *randoms, _ints("tokens_out", tokens_out, rows), _ints("n_out", n_out, n), _ints("drop", drop, n),
               _address("workspace", workspace), _bytes(workspace))
 
