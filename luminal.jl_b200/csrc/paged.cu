@@ -201,6 +201,297 @@ struct StoreParams {
   int* dev_err;
 };
 
+// The 32 features of one group of one row as a lane holds them.
+template <typename T> struct Group;
+template <> struct Group<float> {
+  float4 v[8];
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __ldcs(reinterpret_cast<const float4*>(p) + i);
+  }
+  __device__ __forceinline__ float at(int i) const { const float4& x = v[i >> 2]; return (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w; }
+  // smallest and largest; NaN if there is one
+  __device__ __forceinline__ void range(float& lo, float& hi) const {
+    lo = hi = at(0);
+#pragma unroll
+    for (int i = 1; i < 32; ++i) {
+      asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(at(i)));
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(at(i)));
+    }
+  }
+  static constexpr int kParts = 8;           // of 16 bytes
+  static __device__ __forceinline__ uint4 part(const float (&x)[32], int i) {
+    return make_uint4(__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]), __float_as_uint(x[4 * i + 2]), __float_as_uint(x[4 * i + 3]));
+  }
+};
+template <> struct Group<__nv_bfloat16> {
+  uint32_t w[16];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 x = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+  __device__ __forceinline__ void range(float& lo, float& hi) const {
+    uint32_t a = w[0], b = w[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      asm("min.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(w[i]));
+      asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(b) : "r"(w[i]));
+    }
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(lo) : "f"(__uint_as_float(a << 16)), "f"(__uint_as_float(a & 0xffff0000u)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(hi) : "f"(__uint_as_float(b << 16)), "f"(__uint_as_float(b & 0xffff0000u)));
+  }
+  static constexpr int kParts = 4;
+  static __device__ __forceinline__ uint4 part(const float (&x)[32], int i) {
+    uint32_t u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[8 * i + 2 * k], x[8 * i + 2 * k + 1]);
+      u[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+
+// n of one value: rint of the float32 quotient, 0..15
+__device__ __forceinline__ uint32_t level(float x, float m, float s) {
+  return s > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x - m, s)), 0.f), 15.f) : 0u;
+}
+
+// A group's scale, minimum and levels, as the pairs (feature i % 16 < 8, the one 8 further) that share a byte: byte 8 (i / 16) + i % 8 of `pairs`.  A level is the rint of a
+// float32 quotient; it is formed with the reciprocal, off by less than 1e-5, and by the quotient where that is near a half: for one value of 1500 in bf16, whose quotients are
+// halves that often, so half of the warps have one.
+template <typename T>
+__device__ __forceinline__ void quantise(const Group<T>& x, const T* from, __half& s, __half& m, uint32_t (&pairs)[4]) {
+  float lo, hi;
+  x.range(lo, hi);
+  m = __float2half_rn(lo);
+  s = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+  const float mf = __half2float(m), sf = __half2float(s);
+  if (!(fabsf(mf) <= 65504.f) || !(sf <= 65504.f)) {        // a group without a 4-bit form reads back as NaN
+    m = s = __ushort_as_half(0x7fff);
+    pairs[0] = pairs[1] = pairs[2] = pairs[3] = 0;
+    return;
+  }
+  const float inv = sf > 0.f ? __fdividef(1.f, 15.f * sf) : 0.f;
+  constexpr float kInt = 12582912.f;         // 1.5 2^23: a small number added to it leaves its rint in the low bits
+  uint32_t near_half = 0;                    // bit i: feature i
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t n[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int f = (i >> 1) * 16 + (i & 1) * 4 + (k & 3) + (k >> 2) * 8;
+      const float q = __saturatef((x.at(f) - mf) * inv);                   // of 15 levels
+      const float r = fmaf(q, 15.f, kInt);
+      if (fabsf(fmaf(q, 15.f, kInt - r)) > 0.49999f) near_half |= 1u << f;
+      n[k] = __float_as_uint(r);
+    }
+    uint32_t byte[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) byte[k] = n[k + 4] * 16u + n[k];
+    pairs[i] = __byte_perm(__byte_perm(byte[0], byte[1], 0x0040), __byte_perm(byte[2], byte[3], 0x0040), 0x5410);
+  }
+  while (near_half) {
+    const int f = __ffs(near_half) - 1, shift = 8 * (f & 3) + (f & 8 ? 4 : 0), word = (f >> 4) * 2 + (f >> 2 & 1);
+    near_half &= near_half - 1;
+    const uint32_t n = level(to_f32(from[f]), mf, sf) << shift, keep = ~(15u << shift);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i == word) pairs[i] = (pairs[i] & keep) | n;
+  }
+}
+
+__device__ __forceinline__ uint8_t* block_of(const StoreParams& p, int slot, int head) {
+  return p.pages + (((int64_t)(slot >> p.shift) * p.heads + head) * (1 << (p.shift - 4)) + ((slot & ((1 << p.shift) - 1)) >> 4)) * kv4::block_bytes(p.D);
+}
+
+// A warp has 16 rows and two groups of a head's keys or values, a lane a row's 32 features, so the range needs no exchange.  Where 16 neighbouring rows go to the 16 places of a block, their
+// bytes become words by exchange between lanes and the warp writes whole sectors; other rows write their bytes one by one.  Rows come in windows of 16; a block that begins in a
+// window and goes on into the next belongs to the first.
+template <typename T>
+__global__ void __launch_bounds__(256) append_kernel(const StoreParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int NG = kv4::groups(p.D), halves = (NG + 1) / 2, lane = threadIdx.x & 31, key = lane & 15;
+  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
+  const int64_t per_window = 2ll * p.heads * halves;
+  const int64_t window = task / per_window;
+  const int rest = (int)(task - window * per_window), head = rest / (2 * halves), side = rest / halves & 1, g = (rest % halves) * 2 + (lane >> 4);
+  const int64_t row0 = window * 16;
+  if (row0 >= p.rows) return;
+  // rows row0 - 16 .. row0 + 31: bit i of `follows`: row i + 1 goes to the place behind row i's
+  auto slot_at = [&](int64_t r) { return r >= 0 && r < p.rows ? p.slots[r] : -1; };
+  const int a = slot_at(row0 - 16 + lane), b = slot_at(row0 + 16 + key);
+  const int a_next = __shfl_down_sync(0xffffffffu, a, 1), first_b = __shfl_sync(0xffffffffu, b, 0);
+  const int b_next = __shfl_down_sync(0xffffffffu, b, 1);
+  const int places = p.n_pages << p.shift;
+  const uint64_t follows = (uint64_t)__ballot_sync(0xffffffffu, a >= 0 && (lane == 31 ? first_b : a_next) == a + 1) |
+                           (uint64_t)(__ballot_sync(0xffffffffu, lane < 15 && b >= 0 && b_next == b + 1) & 0x7fffu) << 32;
+  const uint32_t begins = __ballot_sync(0xffffffffu, a >= 0 && (a & 15) == 0 && a < places);
+  uint64_t run = follows;                    // bit i: rows i .. i + 15 follow one another
+  run &= run >> 1;
+  run &= run >> 2;
+  run &= run >> 4;
+  run &= run >> 7;
+  const uint32_t whole = begins & (uint32_t)run;
+  const int mine = whole >> 16 ? __ffs(whole >> 16) - 1 : 16;            // first row of this window whose block is whole
+  const int others = whole & 0xffffu ? __ffs(whole & 0xffffu) - 1 : 0;   // rows below it belong to the last window's block
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool block = pass == 0;
+    const int64_t row = row0 + (block ? mine + key : key);
+    if (block && mine == 16) continue;
+    const bool live = g < NG && (block || (key >= others && key < mine && slot_at(row) >= 0));
+    if (!block && !__any_sync(0xffffffffu, live)) continue;
+    const int slot = slot_at(row);
+    __half s = __ushort_as_half(0), m = s;
+    uint32_t pairs[4] = {0, 0, 0, 0};
+    if (live) {
+      const T* from = reinterpret_cast<const T*>(side ? p.v : p.k) + row * (side ? p.v_stride : p.k_stride) + head * p.D + g * 32;
+      Group<T> x;
+      x.load(from);
+      quantise<T>(x, from, s, m, pairs);
+    }
+    if (block) {
+      uint8_t* out = block_of(p, slot, head);
+      uint32_t w[4];
+      if (side == 0) {
+        // lanes key and key + 8 (xor 8) have the bytes of the same words: words t, tile of row key % 8.  The lower lane makes those of t = 0, 1, the other one t = 2, 3
+        const bool up = key >= 8;
+        // bytes (tile, 2t + e): register 2 tile + t / 2
+        const uint32_t give0 = up ? pairs[0] : pairs[1], give1 = up ? pairs[2] : pairs[3];
+        const uint32_t got0 = __shfl_xor_sync(0xffffffffu, give0, 8), got1 = __shfl_xor_sync(0xffffffffu, give1, 8);
+        const uint32_t keep0 = up ? pairs[1] : pairs[0], keep1 = up ? pairs[3] : pairs[2];
+        const uint32_t l0 = up ? got0 : keep0, h0 = up ? keep0 : got0, l1 = up ? got1 : keep1, h1 = up ? keep1 : got1;
+        w[0] = __byte_perm(l0, h0, 0x5140);              // t even, tile 0: e = 0 of both keys, e = 1 of both
+        w[1] = __byte_perm(l1, h1, 0x5140);              // tile 1
+        w[2] = __byte_perm(l0, h0, 0x7362);              // t odd
+        w[3] = __byte_perm(l1, h1, 0x7362);
+        if (g < NG) *reinterpret_cast<uint4*>(out + g * 256 + (key & 7) * 32 + (up ? 16 : 0)) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        // keys 2t, 2t + 1, 2t + 8, 2t + 9 (xor 1, 8) have the bytes of the same words; each lane makes those of two features d % 8 of both tiles.  First bytes of keys 8 apart,
+        // then of neighbours
+        const bool up = key >= 8, odd = key & 1;
+        const uint32_t give0 = up ? pairs[0] : pairs[1], give1 = up ? pairs[2] : pairs[3];
+        const uint32_t got0 = __shfl_xor_sync(0xffffffffu, give0, 8), got1 = __shfl_xor_sync(0xffffffffu, give1, 8);
+        const uint32_t keep0 = up ? pairs[1] : pairs[0], keep1 = up ? pairs[3] : pairs[2];
+        const uint32_t l0 = up ? got0 : keep0, h0 = up ? keep0 : got0, l1 = up ? got1 : keep1, h1 = up ? keep1 : got1;
+        // features d % 8 = 4 up + 0..3: halfwords (key, key + 8) of features 0, 1 and 2, 3
+        const uint32_t a0 = __byte_perm(l0, h0, 0x5140), a1 = __byte_perm(l0, h0, 0x7362), b0 = __byte_perm(l1, h1, 0x5140), b1 = __byte_perm(l1, h1, 0x7362);
+        const uint32_t sa = odd ? a0 : a1, sb = odd ? b0 : b1;
+        const uint32_t ga = __shfl_xor_sync(0xffffffffu, sa, 1), gb = __shfl_xor_sync(0xffffffffu, sb, 1);
+        const uint32_t ka = odd ? a1 : a0, kb = odd ? b1 : b0;
+        const uint32_t ea = odd ? ga : ka, oa = odd ? ka : ga, eb = odd ? gb : kb, ob = odd ? kb : gb;
+        const int j = (up ? 4 : 0) + (odd ? 2 : 0), t = (key & 7) >> 1;
+        w[0] = __byte_perm(ea, oa, 0x5410);              // feature j, tile 0: keys 2t, 2t + 8, 2t + 1, 2t + 9
+        w[1] = __byte_perm(eb, ob, 0x5410);
+        w[2] = __byte_perm(ea, oa, 0x7632);              // feature j + 1
+        w[3] = __byte_perm(eb, ob, 0x7632);
+        if (g < NG) {
+          uint8_t* to = out + 8 * p.D + g * 256 + (j * 4 + t) * 8;
+          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+          *reinterpret_cast<uint2*>(to + 32) = make_uint2(w[2], w[3]);
+        }
+      }
+      if (g < NG) {
+        __half* meta = reinterpret_cast<__half*>(out + 16 * p.D) + side * p.D;
+        const int at = side ? kv4::value_meta(key, g) : kv4::key_meta(key, g);
+        meta[at] = s;
+        meta[p.D / 2 + at] = m;
+      }
+    } else if (live) {
+      if (slot >= places) {
+        atomicExch(p.dev_err, kv4::kErrPage);
+      } else {
+        const int k16 = slot & 15;
+        uint8_t* out = block_of(p, slot, head);
+        uint8_t* data = out + (side ? 8 * p.D : 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int d = g * 32 + (i >> 3) * 16 + (i & 7);
+          data[side ? kv4::value_byte(k16, d) : kv4::key_byte(k16, d)] = (uint8_t)(pairs[i >> 2] >> 8 * (i & 3));
+        }
+        __half* meta = reinterpret_cast<__half*>(out + 16 * p.D) + side * p.D;
+        const int at = side ? kv4::value_meta(k16, g) : kv4::key_meta(k16, g);
+        meta[at] = s;
+        meta[p.D / 2 + at] = m;
+      }
+    }
+  }
+}
+
+// One thread per row, side, head and group: its bytes lie in one run of 32 bytes (keys) or in 8 bytes of each of 8 (values), which the neighbouring keys' threads read too.
+template <typename T>
+__global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int NG = kv4::groups(p.D), halves = (NG + 1) / 2, lane = threadIdx.x & 31;
+  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
+  const int64_t per_window = 2ll * p.heads * halves;
+  const int64_t window = task / per_window;
+  const int rest = (int)(task - window * per_window), head = rest / (2 * halves), side = rest / halves & 1, g = (rest % halves) * 2 + (lane >> 4);
+  constexpr int kParts = Group<T>::kParts, kPitch = kParts + 1;          // 16-byte pieces of a lane's group, and one to spread the banks
+  __shared__ uint4 staged[8][32 * kPitch];
+  uint4* mine = staged[threadIdx.x >> 5];
+  const int64_t row = window * 16 + (lane & 15);
+  if (window * 16 >= p.rows) return;
+  int slot = row < p.rows && g < NG ? p.slots[row] : -1;
+  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); slot = -1; }
+  const unsigned live = __ballot_sync(0xffffffffu, slot >= 0);
+  if (slot >= 0) {
+  const int key = slot & 15;
+  const uint8_t* block = block_of(p, slot, head);
+  uint32_t pairs[4];                         // as quantise() forms them
+  if (side == 0) {
+    const uint4* src = reinterpret_cast<const uint4*>(block + g * 256 + (key & 7) * 32);
+    const uint4 x = src[0], y = src[1];      // words (t, tile): bytes e = 0 of keys key % 8 and + 8, e = 1
+    const uint32_t pick = key & 8 ? 0x7531 : 0x6420;
+    pairs[0] = __byte_perm(x.x, x.z, pick);
+    pairs[2] = __byte_perm(x.y, x.w, pick);
+    pairs[1] = __byte_perm(y.x, y.z, pick);
+    pairs[3] = __byte_perm(y.y, y.w, pick);
+  } else {
+    const uint8_t* src = block + 8 * p.D + g * 256 + ((key & 7) >> 1) * 8;
+    const int byte = 2 * (key & 1) + (key >> 3);
+    uint2 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const uint2*>(src + j * 32);
+    const uint32_t two = byte | (4 + byte) << 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      pairs[h] = __byte_perm(__byte_perm(x[4 * h].x, x[4 * h + 1].x, two), __byte_perm(x[4 * h + 2].x, x[4 * h + 3].x, two), 0x5410);
+      pairs[2 + h] = __byte_perm(__byte_perm(x[4 * h].y, x[4 * h + 1].y, two), __byte_perm(x[4 * h + 2].y, x[4 * h + 3].y, two), 0x5410);
+    }
+  }
+  const __half* meta = reinterpret_cast<const __half*>(block + 16 * p.D) + side * p.D;
+  const int at = side ? kv4::value_meta(key, g) : kv4::key_meta(key, g);
+  const float s = __half2float(meta[at]), m = __half2float(meta[p.D / 2 + at]);
+  float out[32];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int f = (i >> 3) * 16 + (i & 7);
+    const uint32_t b = pairs[i >> 2] >> 8 * (i & 3);
+    out[f] = fmaf((float)(b & 15u), s, m);
+    out[f + 8] = fmaf((float)(b >> 4 & 15u), s, m);
+  }
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) mine[lane * kPitch + i] = Group<T>::part(out, i);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    const int piece = i * 32 + lane, of = piece / kParts, part = piece - of * kParts;      // lane `of` has row window * 16 + of % 16, group g0 + of / 16
+    if (live >> of & 1) {
+      T* to = reinterpret_cast<T*>(side ? p.v : p.k) + (window * 16 + (of & 15)) * (side ? p.v_stride : p.k_stride) + head * p.D + ((rest % halves) * 2 + (of >> 4)) * 32;
+      reinterpret_cast<uint4*>(to)[part] = mine[of * kPitch + part];
+    }
+  }
+}
+
 template <typename T> struct Pair;           // two neighbouring features
 template <> struct Pair<float> {
   static __device__ __forceinline__ float2 load(const float* p) { return *reinterpret_cast<const float2*>(p); }
@@ -211,14 +502,9 @@ template <> struct Pair<__nv_bfloat16> {
   static __device__ __forceinline__ void store(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y); }
 };
 
-// n of one value: rint of the float32 quotient, 0..15
-__device__ __forceinline__ uint32_t level(float x, float m, float s) {
-  return s > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x - m, s)), 0.f), 15.f) : 0u;
-}
-
-// Eight lanes per row, side, head and group; lane (tile, t) has features 16 tile + 2t, 2t + 1, 2t + 8, 2t + 9, which are two bytes of either form.
+// Few rows: eight lanes per row, side, head and group, a quarter of the work for each; lane (tile, t) has features 16 tile + 2t, 2t + 1, 2t + 8, 2t + 9, which are two bytes of either form.
 template <typename T>
-__global__ void __launch_bounds__(256) append_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(256) append_few_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int NG = kv4::groups(p.D);
@@ -250,7 +536,7 @@ __global__ void __launch_bounds__(256) append_kernel(const StoreParams p) {
   const float mf = __half2float(m), sf = __half2float(s);
   const uint32_t e0 = level(a.x, mf, sf) | level(b.x, mf, sf) << 4, e1 = level(a.y, mf, sf) | level(b.y, mf, sf) << 4;
   const int key = slot & 15;
-  uint8_t* block = p.pages + (((int64_t)(slot >> p.shift) * p.heads + head) * (1 << (p.shift - 4)) + ((slot & ((1 << p.shift) - 1)) >> 4)) * kv4::block_bytes(p.D);
+  uint8_t* block = block_of(p, slot, head);
   uint8_t* data = block + (side ? 8 * p.D : 0);
   const int d = g * 32 + tile * 16 + 2 * t;
   data[side ? kv4::value_byte(key, d) : kv4::key_byte(key, d)] = (uint8_t)e0;
@@ -265,7 +551,7 @@ __global__ void __launch_bounds__(256) append_kernel(const StoreParams p) {
 
 // The same lanes the other way.
 template <typename T>
-__global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(256) read_few_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int NG = kv4::groups(p.D);
@@ -279,7 +565,7 @@ __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
   if (slot < 0) return;
   if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); return; }
   const int key = slot & 15;
-  const uint8_t* block = p.pages + (((int64_t)(slot >> p.shift) * p.heads + head) * (1 << (p.shift - 4)) + ((slot & ((1 << p.shift) - 1)) >> 4)) * kv4::block_bytes(p.D);
+  const uint8_t* block = block_of(p, slot, head);
   const uint8_t* data = block + (side ? 8 * p.D : 0);
   const int d = g * 32 + tile * 16 + 2 * t;
   const uint32_t e0 = data[side ? kv4::value_byte(key, d) : kv4::key_byte(key, d)], e1 = data[side ? kv4::value_byte(key, d + 1) : kv4::key_byte(key, d + 1)];
@@ -333,11 +619,15 @@ int32_t store_params(const char* who, Ctx* ctx, int32_t dtype, const void* k, co
   return LMB200_OK;
 }
 
+// Both ways give the same bits.  The wide one has a quarter of the threads, each with four times the work: below kFewGroups groups its chain is longer than what it saves.
+constexpr int64_t kFewGroups = 24576;
 template <typename K>
-int32_t launch_store(Ctx* ctx, K kernel, const StoreParams& p) {
-  const int64_t threads = (int64_t)p.rows * 2 * p.heads * kv4::groups(p.D) * 8;
+int32_t launch_store(Ctx* ctx, K few, K many, const StoreParams& p) {
+  const int NG = kv4::groups(p.D);
+  const bool wide = (int64_t)p.rows * 2 * p.heads * NG > kFewGroups;
+  const int64_t threads = wide ? ceil_div((int64_t)p.rows, 16) * 2 * p.heads * ((NG + 1) / 2) * 32 : (int64_t)p.rows * 2 * p.heads * NG * 8;
   LMB_REQUIRE(ceil_div(threads, 256) <= INT_MAX, "kv4: %d rows of %d heads are too many for one call", p.rows, p.heads);
-  LMB_CUDA(launch_k_opt(false, kernel, dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, ctx->stream, p));
+  LMB_CUDA(launch_k_opt(false, wide ? many : few, dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
 }
@@ -400,7 +690,7 @@ extern "C" int32_t lmb200_kv4_append(lmb200_ctx h, int32_t dtype, const void* k,
   LMB_TRY(store_params("kv4_append", ctx, dtype, k, v, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
   if (rows == 0) return LMB200_OK;
   LMB_CUDA(cudaSetDevice(ctx->device));
-  return dtype == LMB200_F32 ? launch_store(ctx, append_kernel<float>, p) : launch_store(ctx, append_kernel<__nv_bfloat16>, p);
+  return dtype == LMB200_F32 ? launch_store(ctx, append_few_kernel<float>, append_kernel<float>, p) : launch_store(ctx, append_few_kernel<__nv_bfloat16>, append_kernel<__nv_bfloat16>, p);
 }
 
 extern "C" int32_t lmb200_kv4_read(lmb200_ctx h, int32_t dtype, void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads,
@@ -411,5 +701,5 @@ extern "C" int32_t lmb200_kv4_read(lmb200_ctx h, int32_t dtype, void* k_out, voi
   LMB_TRY(store_params("kv4_read", ctx, dtype, k_out, v_out, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
   if (rows == 0) return LMB200_OK;
   LMB_CUDA(cudaSetDevice(ctx->device));
-  return dtype == LMB200_F32 ? launch_store(ctx, read_kernel<float>, p) : launch_store(ctx, read_kernel<__nv_bfloat16>, p);
+  return dtype == LMB200_F32 ? launch_store(ctx, read_few_kernel<float>, read_kernel<float>, p) : launch_store(ctx, read_few_kernel<__nv_bfloat16>, read_kernel<__nv_bfloat16>, p);
 }

@@ -100,8 +100,8 @@ def store(pages, k, v, slots, page):
                 halves[meta[t] + D // 2] = m[r, h]
 
 
-def load(pages, slots, page, D):
-    """Values [rows, heads, D] in 64 bits of keys and values at slots."""
+def load(pages, slots, page, D, size=False):
+    """Values m + n s [rows, heads, D] in 64 bits of keys and values at slots; with `size` |m| + n s instead."""
     kb, vb, shift, km, vm = places(D)
     out = []
     for byte, meta in ((kb, km), (vb, vm)):
@@ -111,7 +111,8 @@ def load(pages, slots, page, D):
         n = np.take_along_axis(block, np.broadcast_to(byte[t][:, None], block.shape[:2] + (D,)), -1) >> shift[t][:, None] & 15
         halves = block[..., 16 * D:].copy().view(np.float16)
         at = np.broadcast_to(meta[t][:, None], block.shape[:2] + (D // 32,))
-        out.append(values(n, np.take_along_axis(halves, at, -1), np.take_along_axis(halves, at + D // 2, -1)))
+        m = np.take_along_axis(halves, at + D // 2, -1)
+        out.append(values(n, np.take_along_axis(halves, at, -1), np.abs(m) if size else m))
     return out
 
 
@@ -126,10 +127,9 @@ def attention(q, cu, lens, table, pages, page, scale, window=0):
         if new == 0 or held == 0:
             continue
         pos = np.arange(held)
-        k, v = load(pages, table[b, pos // page].astype(np.int64) * page + pos % page, page, D)
-        ak, av = np.abs(k), np.abs(v)
-        # |m| + s n may be larger than |m + s n|
-        kn, vn = ak + 2 * np.abs(np.minimum(k, 0)), av + 2 * np.abs(np.minimum(v, 0))
+        slots = table[b, pos // page].astype(np.int64) * page + pos % page
+        k, v = load(pages, slots, page, D)
+        kn, vn = load(pages, slots, page, D, size=True)
         for t in range(new):
             p0 = held - new + t
             if p0 < 0:

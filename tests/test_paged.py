@@ -827,3 +827,58 @@ def test_calls_at_the_same_time_with_a_workspace_each(lib_built):
         assert all(torch.equal(a, x) for x in o)
     for d in devs:
         d.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,heads,D,page,offset", [(600, 8, 128, 64, 0), (600, 8, 128, 64, 5), (2100, 3, 96, 16, 15), (700, 12, 64, 32, 16), (333, 7, 256, 256, 9), (5000, 8, 32, 128, 1),
+                                                      (512, 9, 160, 16, 0), (4096, 1, 192, 64, 63)])
+def test_append_many_rows(on_torch, dtype, rows, heads, D, page, offset):
+    """Enough rows that whole blocks are written at once: sequences that begin anywhere, end anywhere, rows left out in between, the places around them untouched."""
+    import torch
+    L, dev = on_torch
+    rng = np.random.default_rng(rows + D + offset)
+    tdt = torch.float32 if dtype == "f32" else torch.bfloat16
+    slots, at, n_pages = [], 0, 0
+    while len(slots) < rows:                                   # runs of one sequence each
+        n = int(min(rows - len(slots), rng.choice([1, 3, 15, 16, 17, 40, 200, 700])))
+        first = offset if not slots else int(rng.integers(0, page))
+        pages_of = n_pages + rng.permutation(-(-(first + n) // page))
+        n_pages += len(pages_of)
+        pos = first + np.arange(n)
+        slots += list(pages_of[pos // page] * page + pos % page)
+    slots = np.array(slots, np.int32)
+    slots[rng.random(rows) < 0.01] = -1
+    x = rng.standard_normal((2, rows, heads, D)).astype(np.float32) * 10.0 ** rng.uniform(-3, 3, (2, rows, heads, 1)).astype(np.float32)
+    x[0, 40:56, 0, :32] = np.arange(32) / 2                    # quotients that end in a half
+    x[1, 40:56, 0, :32] = -np.arange(32) / 2
+    x[0, 60, 0, 5], x[0, 61, 0, 31], x[1, 62, 0, 0], x[1, 63, 0, 1], x[1, 64, 0, 1], x[0, 65, 0, 2] = np.nan, np.inf, -np.inf, 7e4, -7e4, 2e6
+    x[1, 70, 0, :32], x[1, 71, 0, :32] = 0, 1.5
+    k, v = cuda(x[0]).to(tdt), cuda(x[1]).to(tdt)
+    start = rng.integers(0, 256, (n_pages, heads, page // 16, 20 * D), dtype=np.uint8)
+    want = start.copy()
+    P.store(want, k.float().cpu().numpy(), v.float().cpu().numpy(), slots, page)
+    pages = cuda(start)
+    L.kv4_append(dev, k, v, cuda(slots), pages, page_size=page)
+    rk, rv = torch.full_like(k, 9.0), torch.full_like(v, 9.0)
+    L.kv4_read(dev, rk, rv, cuda(slots), pages, page_size=page)
+    dev.sync()
+    got = pages.cpu().numpy()
+    assert np.array_equal(got[..., :16 * D], want[..., :16 * D])
+    a, b = got[..., 16 * D:].copy().view(np.uint16), want[..., 16 * D:].copy().view(np.uint16)
+    nan = (a & 0x7fff) > 0x7c00
+    assert np.array_equal(nan, (b & 0x7fff) > 0x7c00) and np.array_equal(a[~nan], b[~nan])
+    live = slots >= 0
+    for r, side in zip((rk, rv), P.load(want, np.where(live, slots, 0), page, D)):
+        with np.errstate(all="ignore"):
+            exact = torch.from_numpy(side.astype(np.float32)).to(tdt)
+        g = r.cpu()
+        assert (g[~live] == 9).all()
+        assert torch.equal(torch.nan_to_num(g[live], nan=3.0e38), torch.nan_to_num(exact[live], nan=3.0e38))
+    # the last slots lie outside a cache of one page less: those rows are left out, and told of
+    short = pages[:n_pages - 1].contiguous()
+    before = short.clone()
+    L.kv4_append(dev, k, v, cuda(slots), short, page_size=page)
+    with pytest.raises(L.LuminalB200Error):
+        dev.sync()
+    assert torch.equal(short[..., :16 * D], before[..., :16 * D])
