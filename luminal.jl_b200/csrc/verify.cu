@@ -4,10 +4,11 @@
 // q = softmax(draft / T) (without draft logits: all of q on t), t is taken where u q(t) < p(t).  The first row that takes nothing, or the last row, gives one new token:
 // the smallest j with sum_{i <= j} w_i > u' sum w, w = max(p - q, 0), and w = p behind the last draft.  T <= 0: the largest logit judges and is given.
 //
-// Two launches.  statistics_kernel reads every row once, split over CTAs, and leaves a maximum and a sum per part.  choose_kernel, a cluster per sequence, joins the parts,
-// finds the row that gives the token and reads that row again (it is in L2) for the sums in 64 bits: where two borders of the running sum lie 1e-6 apart, sums of 32-bit
-// exponentials, off by about 1e-8 of the total, would now and then choose the neighbour of the right token.
-#include <cooperative_groups.h>
+// Launches.  statistics_kernel reads every row once, split over CTAs, and leaves a maximum and a sum per part; decide_kernel joins the parts and finds the row that gives the token.
+// That row is read again (it is in L2) with everything in 64 bits: where two borders of the running sum lie 1e-6 apart, sums of 32-bit exponentials, off by about 1e-8 of
+// the total, would now and then choose the neighbour of the right token.  totals_kernel sums its exponentials over chunks of the vocabulary, weights_kernel the weights where they need
+// those totals (max(p - q, 0)), and choose_kernel finds the chunk and in it the token.  As one kernel with a cluster per sequence the last four took 57 us for 26 sequences of
+// 128256 logits: an SM had CTAs of two sequences or of none, and each of a sequence's eight joined the parts.
 #include <float.h>
 #include <limits.h>
 #include <math_constants.h>
@@ -20,7 +21,7 @@
 namespace lmb {
 namespace {
 
-constexpr int kStatThreads = 256, kChooseThreads = 512, kSplits = 16;
+constexpr int kStatThreads = 256, kChooseThreads = 512, kSplits = 16, kDecideThreads = 128, kMostChunks = 64, kChunk = 2048;
 
 struct VerifyParams {
   const void *target, *draft;
@@ -30,7 +31,12 @@ struct VerifyParams {
   const float *temperature, *accept_u, *sample_u;
   int *tokens_out, *n_out, *drop;
   int* dev_err;
-  float4* part;                              // [rows][kSplits]: target's maximum and sum (or the place of the maximum), draft's
+  int chunks;                                // of the vocabulary
+  float4* part;                              // [rows][kSplits]: target's maximum and sum (T <= 0: the place of the maximum), draft's
+  // of a sequence, at the place of its first row
+  struct Choice* choice;                     // [rows]
+  double2* total;                            // [rows][kMostChunks]: sums of the target's (without a token that is left out) and the draft's exponentials
+  double* weight;                            // [rows][kMostChunks]
 };
 
 // a logit as it counts: NaN is no choice, infinities are the largest number
@@ -39,13 +45,19 @@ __device__ __forceinline__ float clean(float x) { return x == x ? fminf(x, FLT_M
 // log2(e) / T, within what keeps 0 times it and -infinity times it defined
 __device__ __forceinline__ float slope_of(float T) { return fminf(fmaxf(1.4426950408889634f / T, 1e-30f), 1e30f); }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2, float c) {
   const float mn = fmaxf(m, m2), mu = mn == -CUDART_INF_F ? 0.f : mn;
-  s = s * exp2f((m - mu) * c) + s2 * exp2f((m2 - mu) * c);
+  s = s * exp2_fast((m - mu) * c) + s2 * exp2_fast((m2 - mu) * c);
   m = mn;
 }
 __device__ __forceinline__ void join_best(float& m, int& at, float m2, int at2) {
-  if (m2 > m || (m2 == m && at2 < at)) { m = m2; at = at2; }
+  if (m2 > m || (m2 == m && at2 < at && m > -CUDART_INF_F)) { m = m2; at = at2; }
 }
 
 // N neighbouring logits of a row from an aligned place
@@ -70,54 +82,88 @@ template <> struct Run<__nv_bfloat16> {
   }
 };
 
-// f(first, values, count) over this thread's share of part `split` of a row: aligned runs in the middle, single values at the row's ends.
+// f(first, values) over this thread's share of part `split` of a row: aligned runs in the middle, kTogether of them at a time (-infinity where there is none), single values
+// at the row's ends.
+constexpr int kTogether = 4;
 template <typename T, typename F>
 __device__ __forceinline__ void walk(const T* row, int vocab, int split, int splits, F f) {
   constexpr int N = Run<T>::N;
   const int head = min(vocab, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
   const int runs = (vocab - head) / N, tail = head + runs * N;
   const int per = (runs + splits - 1) / splits, r1 = min(runs, (split + 1) * per);
-  float x[N];
-#pragma unroll 2
-  for (int r = split * per + (int)threadIdx.x; r < r1; r += blockDim.x) {
-    Run<T>::load(row + head + r * N, x);
+  float x[kTogether][N];
+  for (int r = split * per + (int)threadIdx.x; r < r1; r += kTogether * kStatThreads) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = clean(x[i]);
-    f(head + r * N, x, N);
+    for (int h = 0; h < kTogether; ++h) {
+      if (r + h * kStatThreads < r1) {
+        Run<T>::load(row + head + (r + h * kStatThreads) * N, x[h]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[h][i] = -CUDART_INF_F;
+      }
+    }
+    f(head + r * N, x);
   }
   if (split == 0) {
     const int ends = head + (vocab - tail);
-    for (int e = threadIdx.x; e < ends; e += blockDim.x) {
+    for (int e = threadIdx.x; e < ends; e += kStatThreads) {
       const int j = e < head ? e : tail + (e - head);
-      x[0] = clean(to_f32(row[j]));
 #pragma unroll
-      for (int i = 1; i < N; ++i) x[i] = -CUDART_INF_F;
-      f(j, x, 1);
+      for (int h = 0; h < kTogether; ++h)
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[h][i] = -CUDART_INF_F;
+      x[0][0] = to_f32(row[j]);
+      f(j, x);
     }
   }
 }
 
+// Maximum and sum of 2^(c (x - maximum)).  Values are taken as they are; where NaN or +infinity made the sum no number, the part is gone through again with every
+// value cleaned.
 template <typename T>
 __device__ __forceinline__ float2 row_stats(const T* row, int vocab, int split, int splits, float c) {
-  float m = -CUDART_INF_F, s = 0.f;
-  walk(row, vocab, split, splits, [&](int, const float* x, int) {
-    float top = x[0];
+  constexpr int N = Run<T>::N;
+  float m, s;
+  auto pass = [&](bool cleaned) {
+    m = -CUDART_INF_F;
+    s = 0.f;
+    walk(row, vocab, split, splits, [&](int, float (&x)[kTogether][N]) {
+      float top = -CUDART_INF_F;
 #pragma unroll
-    for (int i = 1; i < Run<T>::N; ++i) top = fmaxf(top, x[i]);
-    const float mn = fmaxf(m, top), mu = mn == -CUDART_INF_F ? 0.f : mn;
-    s *= exp2f((m - mu) * c);
+      for (int h = 0; h < kTogether; ++h)
 #pragma unroll
-    for (int i = 0; i < Run<T>::N; ++i) s += exp2f((x[i] - mu) * c);
-    m = mn;
-  });
+        for (int i = 0; i < N; ++i) {
+          if (cleaned) x[h][i] = clean(x[h][i]);
+          top = fmaxf(top, x[h][i]);
+        }
+      if (top > m) {
+        s *= exp2_fast((m - top) * c);
+        m = top;
+      }
+      const float mu = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll
+      for (int h = 0; h < kTogether; ++h) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += exp2_fast((x[h][i] - mu) * c);        // (the difference first: T may be tiny)
+        s += sum;
+      }
+    });
+  };
+  pass(false);
+  if (!(s < CUDART_INF_F)) pass(true);
   __shared__ float2 red[kStatThreads / 32];
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) join(m, s, __shfl_xor_sync(0xffffffffu, m, off), __shfl_xor_sync(0xffffffffu, s, off), c);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(m, s);
   __syncthreads();
-  for (int w = 0; w < kStatThreads / 32; ++w)
-    if (w != (int)(threadIdx.x >> 5)) join(m, s, red[w].x, red[w].y, c);
+  if (threadIdx.x >= 32) return make_float2(0.f, 0.f);       // the first warp's is asked for
+  const float2 v = threadIdx.x < kStatThreads / 32 ? red[threadIdx.x] : make_float2(-CUDART_INF_F, 0.f);
+  m = v.x;
+  s = v.y;
+#pragma unroll
+  for (int off = kStatThreads / 64; off > 0; off >>= 1) join(m, s, __shfl_xor_sync(0xffffffffu, m, off), __shfl_xor_sync(0xffffffffu, s, off), c);
   return make_float2(m, s);
 }
 
@@ -154,10 +200,17 @@ __global__ void __launch_bounds__(kStatThreads) statistics_kernel(const VerifyPa
   } else {
     float m = -CUDART_INF_F;
     int at = INT_MAX;
-    walk(target, p.vocab, split, p.splits, [&](int first, const float* x, int) {
+    walk(target, p.vocab, split, p.splits, [&](int first, float (&x)[kTogether][Run<T>::N]) {
 #pragma unroll
-      for (int i = 0; i < Run<T>::N; ++i)
-        if (x[i] > m || (x[i] == m && x[i] > -CUDART_INF_F && first + i < at)) { m = x[i]; at = first + i; }
+      for (int h = 0; h < kTogether; ++h) {
+        float top = x[h][0];
+#pragma unroll
+        for (int i = 1; i < Run<T>::N; ++i) top = fmaxf(top, x[h][i]);
+        if (top > -CUDART_INF_F && top >= m) {               // a new maximum, or an equal one
+#pragma unroll
+          for (int i = 0; i < Run<T>::N; ++i) join_best(m, at, clean(x[h][i]), first + h * kStatThreads * Run<T>::N + i);
+        }
+      }
     });
     __shared__ float2 red[kStatThreads / 32];
 #pragma unroll
@@ -171,42 +224,125 @@ __global__ void __launch_bounds__(kStatThreads) statistics_kernel(const VerifyPa
   if (threadIdx.x == 0) p.part[(int64_t)row * kSplits + split] = out;
 }
 
-__device__ __forceinline__ double block_sum(double v, double* red) {
+// What a sequence's token is chosen from.
+struct Choice {
+  int row;                                   // -1: the token is there
+  int without;                               // token that is left out, or -1
+  int minus;                                 // the draft's probabilities are taken off
+  float top, draft_top;
+};
+
+// exp((x - top) / T) in 64 bits for a logit x <= top: 2^(k / 32) from a table, times a polynomial of 2^f, |f| <= 1 / 64 (its first term left out is 3e-15).
+struct Power {
+  const double* table;                       // [32] in shared memory: 2^(k / 32)
+  double slope, top;                         // log2(e) / T
+  float least;                               // logits below it count for nothing: less than 2^-900 of the top's
+  __device__ __forceinline__ Power(const double* t, float m, double inv_T) : table(t), slope(inv_T * 1.4426950408889634), top(m) {
+    least = (float)fmax(top - 900.0 / slope, -3.4028234e38);
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    asm("min.NaN.f32 %0, %0, 0f7f7fffff;" : "+f"(x));                    // +infinity as the largest float; NaN stays, and fails the comparison
+    if (!(x >= least)) return 0.0;
+    constexpr double kInt = 6755399441055744.0;                          // 1.5 2^52: a small number added to it leaves its rint in the low bits
+    const double y = ((double)x - top) * slope, shifted = fma(y, 32.0, kInt), f = fma(shifted - kInt, -0.03125, y);
+    const int k = __double2loint(shifted);
+    // ln(2)^n / n!
+    const double e = fma(fma(fma(fma(fma(f, 1.3333558146428443e-3, 9.618129107628477e-3), f, 5.550410866482158e-2), f, 0.24022650695910072), f, 0.6931471805599453), f, 1.0) *
+                     table[k & 31];
+    return __hiloint2double(__double2hiint(e) + (k >> 5) * 1048576, __double2loint(e));
+  }
+};
+
+// A chunk of the chosen row: thread's runs of N neighbouring logits, of the target and the draft.
+template <typename T> struct Chunk {
+  static constexpr int N = Run<T>::N;
+  const T *target, *draft;
+  int first, end, vocab;                     // runs
+  bool aligned, minus;
+  __device__ __forceinline__ Chunk(const VerifyParams& p, const Choice& c, int chunk)
+      : target(reinterpret_cast<const T*>(p.target) + c.row * p.target_stride), draft(reinterpret_cast<const T*>(p.draft) + c.row * p.draft_stride), vocab(p.vocab), minus(c.minus) {
+    const int runs = (p.vocab + N - 1) / N, per = (runs + p.chunks - 1) / p.chunks;
+    first = min(runs, chunk * per);
+    end = min(runs, first + per);
+    aligned = (((uintptr_t)target | (minus ? (uintptr_t)draft : 0)) & 15) == 0;
+  }
+  __device__ __forceinline__ void load(int run, float (&a)[N], float (&d)[N]) const {
+    const int j = run * N;
+    if (aligned && run < end && j + N <= vocab) {
+      Run<T>::load(target + j, a);
+      if (minus) Run<T>::load(draft + j, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool there = run < end && j + i < vocab;
+        a[i] = there ? to_f32(target[j + i]) : -CUDART_INF_F;
+        if (minus) d[i] = there ? to_f32(draft[j + i]) : -CUDART_INF_F;
+      }
+    }
+  }
+};
+
+// The weights of a run's tokens.
+template <int N>
+__device__ __forceinline__ void weights_of(const Power& ep, const Power& eq, bool minus, double ip, double iq, int without, int first, const float (&a)[N], const float (&d)[N],
+                                           double (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w[i] = ep(a[i]);
+    if (minus) {                             // (products rounded, so 0 where the two are equal)
+      const double x = __dsub_rn(__dmul_rn(w[i], ip), __dmul_rn(eq(d[i]), iq));
+      w[i] = x > 0.0 ? x : 0.0;
+    } else if (first + i == without) {
+      w[i] = 0.0;
+    }
+  }
+}
+
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+template <int kThreads> __device__ __forceinline__ double block_sum(double v, double* red) {
+  v = warp_sum(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   double s = 0.0;
-  for (int w = 0; w < kChooseThreads / 32; ++w) s += red[w];
+  for (int w = 0; w < kThreads / 32; ++w) s += red[w];
   return s;
 }
+// a sequence's first row; -1: it has none, or rows that are not there
+__device__ __forceinline__ int first_row(const VerifyParams& p, int b) {
+  const int r0 = p.cu_rows[b], r1 = p.cu_rows[b + 1];
+  return r0 < 0 || r1 > p.rows || r1 <= r0 ? -1 : r0;
+}
+__device__ __forceinline__ double inverse_T(const VerifyParams& p, int b) { return fmin(fmax(1.0 / (double)p.temperature[b], 1e-30), 1e30); }
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+}
 
+// One CTA per sequence, a warp per row: which drafts are taken, and what the next token is chosen from.
 template <typename T>
-__global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyParams p) {
-  namespace cg = cooperative_groups;
-  constexpr int kWarps = kChooseThreads / 32;
+__global__ void __launch_bounds__(kDecideThreads) decide_kernel(const VerifyParams p) {
+  constexpr int kWarps = kDecideThreads / 32;
   __shared__ int stop_row;
-  __shared__ double red[kWarps], of_warp[kWarps];
-  __shared__ double cta[4];                  // this CTA's sums, read by its cluster
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r0 = first_row(p, b), r1 = p.cu_rows[b + 1];     // (no kernel before this one writes what is read in front of the wait)
+  if (tid == 0) stop_row = r1 - 1;
   pdl_launch_dependents();
   pdl_wait();
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r0 = p.cu_rows[b], r1 = p.cu_rows[b + 1];
-  if (r0 < 0 || r1 > p.rows || r1 <= r0) {   // no row of its own, or rows that are not there: the same for the whole cluster
-    if (rank == 0 && tid == 0) {
+  if (r0 < 0) {
+    if (tid == 0) {
       p.n_out[b] = 0;
       p.drop[b] = 0;
-      if (r1 != r0) atomicExch(p.dev_err, kv4::kErrPage);
+      if (r1 != p.cu_rows[b]) atomicExch(p.dev_err, kv4::kErrPage);
     }
     return;
   }
   const float temperature = p.temperature ? p.temperature[b] : 0.f;
   const bool greedy = !(temperature > 0.f);
-  const double inv_T = greedy ? 1.0 : fmin(fmax(1.0 / (double)temperature, 1e-30), 1e30);
-  if (tid == 0) stop_row = r1 - 1;
+  const double slope = greedy ? 1.0 : inverse_T(p, b) * 1.4426950408889634;
   __syncthreads();
   // the parts of a row, joined by a warp; a refused draft ends the sequence there
   auto joined = [&](int row, float& m, double& s, float& md, double& sd) {
@@ -218,13 +354,8 @@ __global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyPara
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
       md = fmaxf(md, __shfl_xor_sync(0xffffffffu, md, off));
     }
-    s = v.x == -CUDART_INF_F ? 0.0 : (double)v.y * exp(((double)v.x - m) * inv_T);
-    sd = v.z == -CUDART_INF_F ? 0.0 : (double)v.w * exp(((double)v.z - md) * inv_T);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, off);
-      sd += __shfl_xor_sync(0xffffffffu, sd, off);
-    }
+    s = warp_sum(v.x == -CUDART_INF_F ? 0.0 : (double)v.y * exp2(((double)v.x - m) * slope));
+    sd = warp_sum(v.z == -CUDART_INF_F ? 0.0 : (double)v.w * exp2(((double)v.z - md) * slope));
   };
   auto best_of = [&](int row, float& m) {
     const float4 v = lane < p.splits ? p.part[(int64_t)row * kSplits + lane] : make_float4(-CUDART_INF_F, __int_as_float(INT_MAX), 0.f, 0.f);
@@ -244,154 +375,227 @@ __global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyPara
     } else {
       float m, md;
       double s, sd;
-      joined(row, m, s, md, sd);
       const bool known = t >= 0 && t < p.vocab;
-      const float l = known ? logit(p.target, p.target_stride, row, t) : -CUDART_INF_F;
-      const double pt = l == -CUDART_INF_F ? 0.0 : exp(((double)l - m) * inv_T) / s;
-      double qt = 1.0;
-      if (p.draft) {
-        const float ld = known ? logit(p.draft, p.draft_stride, row, t) : -CUDART_INF_F;
-        qt = ld == -CUDART_INF_F ? 0.0 : exp(((double)ld - md) * inv_T) / sd;
-      }
+      const float l = known ? logit(p.target, p.target_stride, row, t) : -CUDART_INF_F, ld = known && p.draft ? logit(p.draft, p.draft_stride, row, t) : -CUDART_INF_F;
+      joined(row, m, s, md, sd);
+      const double pt = l == -CUDART_INF_F ? 0.0 : exp2(((double)l - m) * slope) / s;
+      const double qt = !p.draft ? 1.0 : ld == -CUDART_INF_F ? 0.0 : exp2(((double)ld - md) * slope) / sd;
       takes = (double)p.accept_u[row] * qt < pt;
     }
     if (lane == 0 && !takes) atomicMin(&stop_row, row);
   }
   __syncthreads();
   const int stop = stop_row;
-  if (rank == 0) {
-    for (int row = r0 + tid; row < r1; row += kChooseThreads)
-      if (row != stop) p.tokens_out[row] = row < stop ? p.tokens[row + 1] : -1;
-    if (tid == 0) { p.n_out[b] = stop - r0 + 1; p.drop[b] = r1 - 1 - stop; }
-  }
-  if (greedy) {
-    if (rank == 0 && warp == 0) {
-      float m;
-      const int at = best_of(stop, m);
-      if (lane == 0) p.tokens_out[stop] = m > -CUDART_INF_F ? at : -1;
+  if (warp == 0) {
+    Choice c = {stop, -1, 0, -CUDART_INF_F, -CUDART_INF_F};
+    int token = -1;
+    if (greedy) {
+      const int at = best_of(stop, c.top);
+      if (c.top > -CUDART_INF_F) token = at;
+      c.row = -1;
+    } else {
+      double s, sd;
+      joined(stop, c.top, s, c.draft_top, sd);
+      const bool last = stop == r1 - 1;
+      c.minus = !last && p.draft && c.draft_top > -CUDART_INF_F;
+      if (!last && !p.draft) c.without = p.tokens[stop + 1];
+      if (c.top == -CUDART_INF_F) c.row = -1;                // nothing can be chosen
     }
-    return;
-  }
-  float m, md;
-  double s32, sd32;
-  joined(stop, m, s32, md, sd32);
-  if (m == -CUDART_INF_F) {                  // nothing can be chosen
-    if (rank == 0 && tid == 0) p.tokens_out[stop] = -1;
-    return;
-  }
-  const bool last = stop == r1 - 1;
-  bool minus = !last && p.draft && md > -CUDART_INF_F;
-  const int without = !last && !p.draft ? p.tokens[stop + 1] : -1;
-  const T* target = reinterpret_cast<const T*>(p.target) + stop * p.target_stride;
-  const T* draft = reinterpret_cast<const T*>(p.draft) + stop * p.draft_stride;
-  // CTA `rank` has the tokens [first, end), a warp neighbours among them, a lane neighbours among those
-  const int per_cta = (p.vocab + C - 1) / C, per_warp = (per_cta + kWarps - 1) / kWarps;
-  const int c0 = min(p.vocab, rank * per_cta), c1 = min(p.vocab, c0 + per_cta);
-  const int w0 = min(c1, c0 + warp * per_warp), w1 = min(c1, w0 + per_warp);
-  auto ep = [&](int j) { return exp(((double)clean(to_f32(target[j])) - m) * inv_T); };
-  auto eq = [&](int j) { return exp(((double)clean(to_f32(draft[j])) - md) * inv_T); };
-  double ip = 1.0, iq = 0.0;
-  if (minus) {
-    double sp = 0.0, sq = 0.0;
-    for (int j = w0 + lane; j < w1; j += 32) { sp += ep(j); sq += eq(j); }
-    sp = block_sum(sp, red);
-    sq = block_sum(sq, red);
-    if (tid == 0) { cta[0] = sp; cta[1] = sq; }
-    cluster.sync();
-    sp = sq = 0.0;
-    for (int k = 0; k < C; ++k) {
-      const double* o = cluster.map_shared_rank(cta, k);
-      sp += o[0];
-      sq += o[1];
+    if (lane == 0) {
+      p.choice[r0] = c;
+      if (c.row < 0) p.tokens_out[stop] = token;
+      p.n_out[b] = stop - r0 + 1;
+      p.drop[b] = r1 - 1 - stop;
     }
-    ip = 1.0 / sp;
-    iq = 1.0 / sq;
   }
-  int plain = without >= 0 || minus ? 0 : 1; // 1: w = p
-  for (;;) {
-    auto weight = [&](int j) {
-      const double e = ep(j);
-      if (plain) return e;
-      if (minus) return fmax(__dsub_rn(__dmul_rn(e, ip), __dmul_rn(eq(j), iq)), 0.0);   // 0 where the two are equal
-      return j == without ? 0.0 : e;
-    };
-    double mine = 0.0;
-    for (int j = w0 + lane; j < w1; j += 32) mine += weight(j);
+  for (int row = r0 + tid; row < r1; row += kDecideThreads)
+    if (row != stop) p.tokens_out[row] = row < stop ? p.tokens[row + 1] : -1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kStatThreads) totals_kernel(const VerifyParams p) {
+  constexpr int N = Run<T>::N;
+  __shared__ double red[kStatThreads / 32], table[32];
+  fill_table(table);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
+  const int r0 = first_row(p, b);
+  if (r0 < 0) return;
+  const Choice c = p.choice[r0];
+  if (c.row < 0) return;
+  const double inv_T = inverse_T(p, b);
+  __syncthreads();
+  const Chunk<T> chunk_of(p, c, chunk);
+  const Power ep(table, c.top, inv_T), eq(table, c.minus ? c.draft_top : 0.f, inv_T);
+  double sp = 0.0, sq = 0.0;
+  for (int run = chunk_of.first + tid; run < chunk_of.end; run += 2 * kStatThreads) {
+    float a[2][N], d[2][N];
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
-    if (lane == 0) of_warp[warp] = mine;
+    for (int h = 0; h < 2; ++h) chunk_of.load(run + h * kStatThreads, a[h], d[h]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const double e = ep(a[h][i]);
+        if (c.minus) sq += eq(d[h][i]);
+        if ((run + h * kStatThreads) * N + i != c.without) sp += e;
+      }
+  }
+  sp = block_sum<kStatThreads>(sp, red);
+  if (c.minus) sq = block_sum<kStatThreads>(sq, red);
+  if (tid == 0) p.total[(int64_t)r0 * kMostChunks + chunk] = make_double2(sp, sq);
+}
+
+// sums over a sequence's chunks, by a whole warp
+__device__ __forceinline__ double2 totals_of(const VerifyParams& p, int r0) {
+  double sp = 0.0, sq = 0.0;
+  for (int k = threadIdx.x & 31; k < p.chunks; k += 32) {
+    const double2 v = p.total[(int64_t)r0 * kMostChunks + k];
+    sp += v.x;
+    sq += v.y;
+  }
+  return make_double2(warp_sum(sp), warp_sum(sq));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kStatThreads) weights_kernel(const VerifyParams p) {
+  constexpr int N = Run<T>::N;
+  __shared__ double red[kStatThreads / 32], table[32];
+  fill_table(table);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.y, chunk = blockIdx.x;
+  const int r0 = first_row(p, b);
+  if (r0 < 0) return;
+  const Choice c = p.choice[r0];
+  if (c.row < 0 || !c.minus) return;         // else the totals are the weights' own
+  const Chunk<T> chunk_of(p, c, chunk);
+  const double inv_T = inverse_T(p, b);
+  const double2 total = totals_of(p, r0);
+  __syncthreads();
+  const Power ep(table, c.top, inv_T), eq(table, c.draft_top, inv_T);
+  const double ip = 1.0 / total.x, iq = 1.0 / total.y;
+  double sum = 0.0;
+  for (int run = chunk_of.first + (int)threadIdx.x; run < chunk_of.end; run += kStatThreads) {
+    float a[N], d[N];
+    double w[N];
+    chunk_of.load(run, a, d);
+    weights_of<N>(ep, eq, true, ip, iq, -1, run * N, a, d, w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += w[i];
+  }
+  sum = block_sum<kStatThreads>(sum, red);
+  if (threadIdx.x == 0) p.weight[(int64_t)r0 * kMostChunks + chunk] = sum;
+}
+
+// One CTA per sequence: the chunk in which the running sum passes its goal, then the token.  By rounding there may be none; then the last with any weight.
+template <typename T>
+__global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyParams p) {
+  constexpr int kWarps = kChooseThreads / 32, N = Run<T>::N;
+  __shared__ double table[32], of_warp[kWarps];
+  __shared__ int token;
+  fill_table(table);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r0 = first_row(p, b);
+  if (r0 < 0) return;
+  Choice c = p.choice[r0];
+  if (c.row < 0) return;
+  const double inv_T = inverse_T(p, b);
+  const double2 total = totals_of(p, r0);
+  // A lane has two neighbouring chunks.  p <= q everywhere, or nothing but the refused draft: the target itself.  (Where a token was left out, it is not in the totals.)
+  static_assert(kMostChunks == 64, "two chunks a lane");
+  double v0, v1, sum;
+  for (bool again = false;; again = true) {
+    auto at = [&](int k) { return k >= p.chunks ? 0.0 : c.minus ? p.weight[(int64_t)r0 * kMostChunks + k] : p.total[(int64_t)r0 * kMostChunks + k].x; };
+    v0 = at(2 * lane);
+    v1 = at(2 * lane + 1);
+    sum = warp_sum(v0 + v1);
+    if (sum > 0.0 || again || !c.minus) break;
+    c.minus = 0;
+  }
+  if (!(sum > 0.0)) {
+    if (tid == 0) p.tokens_out[c.row] = c.without;
+    return;
+  }
+  const double goal = (double)p.sample_u[b] * sum;
+  double before = v0 + v1;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += x;
+  }
+  const unsigned passing = __ballot_sync(0xffffffffu, v0 + v1 > 0.0 && before > goal), having = __ballot_sync(0xffffffffu, v0 + v1 > 0.0);
+  const int who = passing ? __ffs(passing) - 1 : 31 - __clz(having);
+  before -= v0 + v1;
+  int chunk = 2 * lane;
+  if (!(v0 > 0.0) || (v1 > 0.0 && !(before + v0 > goal))) { before += v0; ++chunk; }
+  chunk = __shfl_sync(0xffffffffu, chunk, who);
+  before = __shfl_sync(0xffffffffu, before, who);
+  __syncthreads();                           // the table
+  const Chunk<T> chunk_of(p, c, chunk);
+  const Power ep(table, c.top, inv_T), eq(table, c.minus ? c.draft_top : 0.f, inv_T);
+  const double ip = 1.0 / total.x, iq = 1.0 / total.y;
+  if (tid == 0) token = -1;
+  for (int base = chunk_of.first; base < chunk_of.end; base += kChooseThreads) {
+    const int run = base + tid;
+    float a[N], d[N];
+    double w[N], v = 0.0;
+    chunk_of.load(run, a, d);
+    weights_of<N>(ep, eq, c.minus, ip, iq, c.without, run * N, a, d, w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v += w[i];
+    double incl = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += x;
+    }
     __syncthreads();
-    if (tid == 0) {
-      double v = 0.0;
-      for (int w = 0; w < kWarps; ++w) v += of_warp[w];
-      cta[2 + plain] = v;
-    }
-    cluster.sync();
-    double total = 0.0;
-    for (int k = 0; k < C; ++k) total += *cluster.map_shared_rank(cta + 2 + plain, k);
-    if (!(total > 0.0) && !plain) { plain = 1; continue; }             // p <= q everywhere: the target itself
-    const double goal = (double)p.sample_u[b] * total;
-    // the first part whose running sum passes the goal; by rounding there may be none, then the last with any weight
-    double run = 0.0, before = 0.0;
-    int at = 0;
-    for (int k = 0; k < C; ++k) {
-      const double v = *cluster.map_shared_rank(cta + 2 + plain, k);
-      if (v > 0.0) { at = k; before = run; if (run + v > goal) break; }
-      run += v;
-    }
-    if (at == rank) {
-      int aw = 0;
-      run = before;
-      for (int w = 0; w < kWarps; ++w) {
-        const double v = of_warp[w];
-        if (v > 0.0) { aw = w; before = run; if (run + v > goal) break; }
-        run += v;
-      }
-      if (aw == warp) {                      // lanes take neighbouring runs of the warp's tokens
-        const int per = (w1 - w0 + 31) / 32, l0 = min(w1, w0 + lane * per), l1 = min(w1, l0 + per);
-        double v = 0.0;
-        for (int j = l0; j < l1; ++j) v += weight(j);
-        double incl = v;
+    if (lane == 31) of_warp[warp] = incl;
+    __syncthreads();
+    double mine = before + incl - v;         // in front of this run
+    for (int k = 0; k < warp; ++k) mine += of_warp[k];
+    for (int k = 0; k < kWarps; ++k) before += of_warp[k];
+    // the first run that passes has the token; without one the last run with any weight, so far
+    const bool passes = v > 0.0 && mine + v > goal;
+    __shared__ int first_pass, last_some;
+    if (tid == 0) { first_pass = INT_MAX; last_some = -1; }
+    __syncthreads();
+    if (passes) atomicMin(&first_pass, run);
+    if (v > 0.0) atomicMax(&last_some, run);
+    __syncthreads();
+    if (run == (first_pass != INT_MAX ? first_pass : last_some)) {
+      bool done = false;
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const double u = __shfl_up_sync(0xffffffffu, incl, off);
-          if (lane >= off) incl += u;
-        }
-        const unsigned passes = __ballot_sync(0xffffffffu, v > 0.0 && before + incl > goal), some = __ballot_sync(0xffffffffu, v > 0.0);
-        const int who = passes ? __ffs(passes) - 1 : 31 - __clz(some);
-        if (lane == who) {
-          double sum = before + incl - v;
-          int chosen = l0;
-          for (int j = l0; j < l1; ++j) {
-            const double wj = weight(j);
-            sum += wj;
-            if (wj > 0.0) { chosen = j; if (sum > goal) break; }
-          }
-          p.tokens_out[stop] = chosen;
-        }
+      for (int i = 0; i < N; ++i) {
+        mine += w[i];
+        if (w[i] > 0.0 && !done) { token = run * N + i; done = mine > goal; }
       }
     }
-    break;
+    if (first_pass != INT_MAX) break;
   }
-  cluster.sync();                            // no CTA leaves while others read its sums
+  __syncthreads();
+  if (tid == 0) p.tokens_out[c.row] = token;
 }
 
 template <typename T>
 int32_t launch_verify(Ctx* ctx, const VerifyParams& p) {
   LMB_CUDA(launch_k_opt(false, statistics_kernel<T>, dim3((unsigned)p.splits, (unsigned)p.rows), dim3(kStatThreads), 0, ctx->stream, p));
   ctx->launches++;
-  const int C = p.vocab <= 4096 ? 1 : 8;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.n_seq * C));
-  cfg.blockDim = dim3(kChooseThreads);
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)C;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  LMB_CUDA(cudaLaunchKernelEx(&cfg, choose_kernel<T>, p));
+  const dim3 grid((unsigned)p.chunks, (unsigned)p.n_seq);
+  LMB_CUDA(launch_k(decide_kernel<T>, dim3((unsigned)p.n_seq), dim3(kDecideThreads), 0, ctx->stream, p));
+  ctx->launches++;
+  if (!p.temperature) return LMB200_OK;      // the tokens are there
+  LMB_CUDA(launch_k(totals_kernel<T>, grid, dim3(kStatThreads), 0, ctx->stream, p));
+  ctx->launches++;
+  if (p.draft) {
+    LMB_CUDA(launch_k(weights_kernel<T>, grid, dim3(kStatThreads), 0, ctx->stream, p));
+    ctx->launches++;
+  }
+  LMB_CUDA(launch_k(choose_kernel<T>, dim3((unsigned)p.n_seq), dim3(kChooseThreads), 0, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
 }
@@ -401,9 +605,10 @@ int32_t launch_verify(Ctx* ctx, const VerifyParams& p) {
 
 using namespace lmb;
 
+// A sequence that has work has a row, so its place in the workspace is its first row's.
 extern "C" int32_t lmb200_verify_drafts_workspace(int32_t rows, int64_t* bytes) {
   LMB_REQUIRE(bytes && rows >= 0, "verify_drafts_workspace: bad argument");
-  *bytes = std::max<int64_t>(16, (int64_t)rows * kSplits * (int64_t)sizeof(float4));
+  *bytes = std::max<int64_t>(16, (int64_t)rows * (kSplits * sizeof(float4) + kMostChunks * (sizeof(double2) + sizeof(double)) + 32));
   return LMB200_OK;
 }
 
@@ -432,6 +637,10 @@ extern "C" int32_t lmb200_verify_drafts(lmb200_ctx h, int32_t dtype, const void*
     return LMB200_OK;
   }
   VerifyParams p = {target, draft, target_stride, draft_stride, vocab, rows, n_seq, vocab <= 4096 ? 1 : kSplits, cu_rows, tokens, temperature, accept_u, sample_u,
-                    tokens_out, n_out, drop, ctx->dev_err, static_cast<float4*>(workspace)};
+                    tokens_out, n_out, drop, ctx->dev_err, (int)std::min<int64_t>(kMostChunks, ceil_div(vocab, kChunk))};
+  p.part = static_cast<float4*>(workspace);
+  p.total = reinterpret_cast<double2*>(p.part + (int64_t)rows * kSplits);
+  p.weight = reinterpret_cast<double*>(p.total + (int64_t)rows * kMostChunks);
+  p.choice = reinterpret_cast<Choice*>(p.weight + (int64_t)rows * kMostChunks);
   return dtype == LMB200_F32 ? launch_verify<float>(ctx, p) : launch_verify<__nv_bfloat16>(ctx, p);
 }
