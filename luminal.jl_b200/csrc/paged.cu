@@ -8,6 +8,7 @@ namespace lmb {
 namespace {
 
 constexpr int kTableThreads = 1024;
+int g_most_ctas = 8;                         // of reserve_kernel's cluster
 constexpr int kMaxSeqs = 8192;               // three words of shared memory each
 
 struct TableParams {
@@ -57,14 +58,17 @@ __device__ __forceinline__ void scan2(long long a, long long b, long long& ea, l
 __device__ __forceinline__ int last_at_most(const int* at, int lo, int hi, int x) {
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (at[mid] <= x) lo = mid; else hi = mid - 1;
+    const bool up = at[mid] <= x;
+    lo = up ? mid : lo;
+    hi = up ? hi : mid - 1;
   }
   return lo;
 }
 
 // One cluster.  Every CTA reads all lengths and forms the same sums (a thread takes neighbouring sequences); behind the cluster's barrier, when
 // nobody reads them any more, the outputs, which may be the inputs' arrays, are written.  Rows and pages are dealt out to all warps in groups
-// of 32 neighbours, whose sequence is found by bisection.
+// of 32 neighbours, whose sequence is found by bisection: what it takes is the chain of those searches and loads, so it wants many warps.  77000 rows of 2048 sequences on 1, 2, 4, 8, 16
+// CTAs: 88, 48, 28, 17, 13 us; 26000 rows of 256: 19, 13, 9.6, 6.9, 6.8.
 __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const TableParams p) {
   extern __shared__ int sm[];
   int* len = sm;
@@ -103,28 +107,49 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const TableParam
   const int n_rows = bad ? 0 : (int)tr, n_new = bad ? 0 : (int)tp;
   const int lane = tid & 31, warps = kTableThreads / 32 * cluster_size(), warp = cluster_rank() * (kTableThreads / 32) + (tid >> 5);
   // slots: the token's page is a new one, or the last that its sequence holds.  (`table` is read at places that this call does not write.)
-  for (int r0 = warp * 32; r0 < p.rows; r0 += warps * 32) {
-    const int r = r0 + lane;
-    int slot = -1;
-    if (r0 < n_rows) {
-      const int lo = last_at_most(row0, 0, p.n_seq - 1, r0);
-      const int hi = last_at_most(row0, lo, p.n_seq - 1, min(r0 + 31, n_rows - 1));
+  // Four groups of 32 at a time, so that their searches and loads overlap.
+  constexpr int kTogether = 4;
+  for (int r00 = warp * 32; r00 < p.rows; r00 += kTogether * warps * 32) {
+    int lo[kTogether], hi[kTogether], seq[kTogether], page[kTogether], pos[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {    // the sequences of a group's first and last row, between which its rows' lie
+      const int r0 = min(r00 + i * warps * 32, max(0, n_rows - 1));
+      lo[i] = last_at_most(row0, 0, p.n_seq - 1, lane == 0 ? r0 : min(r0 + 31, max(0, n_rows - 1)));       // lane 0: first, the others: last
+      hi[i] = __shfl_sync(0xffffffffu, lo[i], 1);
+      lo[i] = __shfl_sync(0xffffffffu, lo[i], 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int r = r00 + i * warps * 32 + lane;
+      page[i] = -1;
       if (r < n_rows) {
-        const int b = lo == hi ? lo : last_at_most(row0, lo, hi, r);
-        const int pos = len[b] + (r - row0[b]);
-        const int j = (pos >> p.shift) - ((len[b] + size1) >> p.shift);
-        const int page = j >= 0 ? p.free_list[free_now - 1 - (page0[b] + j)] : p.table[(int64_t)b * p.max_pages + (pos >> p.shift)];
-        if ((unsigned)page < (unsigned)p.n_pages) slot = (page << p.shift) + (pos & size1);
+        const int b = lo[i] == hi[i] ? lo[i] : last_at_most(row0, lo[i], hi[i], r);
+        pos[i] = len[b] + (r - row0[b]);
+        const int j = (pos[i] >> p.shift) - ((len[b] + size1) >> p.shift);
+        page[i] = j >= 0 ? p.free_list[free_now - 1 - (page0[b] + j)] : p.table[(int64_t)b * p.max_pages + (pos[i] >> p.shift)];
+      }
+      seq[i] = r;
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i)
+      if (seq[i] < p.rows) p.slots[seq[i]] = (unsigned)page[i] < (unsigned)p.n_pages ? (page[i] << p.shift) + (pos[i] & size1) : -1;
+  }
+  for (int k0 = warp * 32; k0 < n_new; k0 += kTogether * warps * 32) {
+    int id[kTogether];
+    int64_t to[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int k = k0 + i * warps * 32 + lane;
+      to[i] = -1;
+      if (k < n_new) {
+        const int b = last_at_most(page0, 0, p.n_seq - 1, k);
+        to[i] = (int64_t)b * p.max_pages + ((len[b] + size1) >> p.shift) + (k - page0[b]);
+        id[i] = p.free_list[free_now - 1 - k];
       }
     }
-    if (r < p.rows) p.slots[r] = slot;
-  }
-  for (int k0 = warp * 32; k0 < n_new; k0 += warps * 32) {
-    const int k = k0 + lane;
-    if (k < n_new) {
-      const int b = last_at_most(page0, 0, p.n_seq - 1, k);
-      p.table[(int64_t)b * p.max_pages + ((len[b] + size1) >> p.shift) + (k - page0[b])] = p.free_list[free_now - 1 - k];
-    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i)
+      if (to[i] >= 0) p.table[to[i]] = id[i];
   }
   if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();   // lens and n_free are read by no one any more
   if (cluster_rank() != 0) return;
@@ -638,6 +663,21 @@ int32_t paged_configure() {
   const int smem = kMaxSeqs * 3 * 4;
   LMB_CUDA(cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   LMB_CUDA(cudaFuncSetAttribute(shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // 16 CTAs are one cluster where the GPU has room for it
+  LMB_CUDA(cudaFuncSetAttribute(reserve_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(kTableThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, reserve_kernel, &cfg) == cudaSuccess && clusters >= 1) g_most_ctas = 16;
+  else cudaGetLastError();
   return LMB200_OK;
 }
 
@@ -663,7 +703,7 @@ extern "C" int32_t lmb200_kv_reserve(lmb200_ctx h, int32_t n_seq, int32_t page_s
   LMB_CUDA(cudaSetDevice(ctx->device));
   TableParams p = {n_seq, kv4::page_shift(page_size), max_pages, n_pages, rows, lens, add, n_free, table, const_cast<int32_t*>(free_list),
                    lens_out, n_free_out, cu_rows, slots, status, ctx->dev_err};
-  LMB_CUDA(launch_cluster(reserve_kernel, n_seq > 512 || rows > 4096 ? 8 : 1, (size_t)n_seq * 12, ctx->stream, p));
+  LMB_CUDA(launch_cluster(reserve_kernel, n_seq <= 512 && rows <= 2048 ? 1 : rows <= 32768 ? 8 : g_most_ctas, (size_t)n_seq * 12, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
 }

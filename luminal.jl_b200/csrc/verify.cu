@@ -7,8 +7,9 @@
 // Launches.  statistics_kernel reads every row once, split over CTAs, and leaves a maximum and a sum per part; decide_kernel joins the parts and finds the row that gives the token.
 // That row is read again (it is in L2) with everything in 64 bits: where two borders of the running sum lie 1e-6 apart, sums of 32-bit exponentials, off by about 1e-8 of
 // the total, would now and then choose the neighbour of the right token.  totals_kernel sums its exponentials over chunks of the vocabulary, weights_kernel the weights where they need
-// those totals (max(p - q, 0)), and choose_kernel finds the chunk and in it the token.  As one kernel with a cluster per sequence the last four took 57 us for 26 sequences of
-// 128256 logits: an SM had CTAs of two sequences or of none, and each of a sequence's eight joined the parts.
+// those totals (max(p - q, 0)), and choose_kernel finds the chunk and in it the token.  at_once_kernel does the last four in one launch with a cluster per sequence: quicker for
+// small vocabularies, slower for large ones, of which an SM gets two sequences or none.
+#include <cooperative_groups.h>
 #include <float.h>
 #include <limits.h>
 #include <math_constants.h>
@@ -22,6 +23,9 @@ namespace lmb {
 namespace {
 
 constexpr int kStatThreads = 256, kChooseThreads = 512, kSplits = 16, kDecideThreads = 128, kMostChunks = 64, kChunk = 2048;
+// Vocabularies up to this size take two launches, larger ones four or five.  One sequence of five rows: 32064 logits 15.5 against 16.9 us, 128256 39.7 against 22.9; 32 sequences: 32064
+// 35.9 against 39.7, 128256 83 against 63.
+constexpr int kAtOnce = 40960;
 
 struct VerifyParams {
   const void *target, *draft;
@@ -322,24 +326,15 @@ __device__ __forceinline__ void fill_table(double* table) {
   if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
 }
 
-// One CTA per sequence, a warp per row: which drafts are taken, and what the next token is chosen from.
-template <typename T>
-__global__ void __launch_bounds__(kDecideThreads) decide_kernel(const VerifyParams p) {
-  constexpr int kWarps = kDecideThreads / 32;
+// A block finds out which drafts of sequence b (rows r0 to r1 - 1) are taken, and what the next token is chosen from (by all threads known at the end); `writes`: and writes
+// down what is known.  A warp per row.
+template <typename T, int kThreads>
+__device__ __forceinline__ Choice decide(const VerifyParams& p, int b, int r0, int r1, bool writes) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ int stop_row;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r0 = first_row(p, b), r1 = p.cu_rows[b + 1];     // (no kernel before this one writes what is read in front of the wait)
+  __shared__ Choice found;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) stop_row = r1 - 1;
-  pdl_launch_dependents();
-  pdl_wait();
-  if (r0 < 0) {
-    if (tid == 0) {
-      p.n_out[b] = 0;
-      p.drop[b] = 0;
-      if (r1 != p.cu_rows[b]) atomicExch(p.dev_err, kv4::kErrPage);
-    }
-    return;
-  }
   const float temperature = p.temperature ? p.temperature[b] : 0.f;
   const bool greedy = !(temperature > 0.f);
   const double slope = greedy ? 1.0 : inverse_T(p, b) * 1.4426950408889634;
@@ -402,82 +397,68 @@ __global__ void __launch_bounds__(kDecideThreads) decide_kernel(const VerifyPara
       if (c.top == -CUDART_INF_F) c.row = -1;                // nothing can be chosen
     }
     if (lane == 0) {
-      p.choice[r0] = c;
-      if (c.row < 0) p.tokens_out[stop] = token;
-      p.n_out[b] = stop - r0 + 1;
-      p.drop[b] = r1 - 1 - stop;
+      found = c;
+      if (writes) {
+        if (c.row < 0) p.tokens_out[stop] = token;
+        p.n_out[b] = stop - r0 + 1;
+        p.drop[b] = r1 - 1 - stop;
+      }
     }
   }
-  for (int row = r0 + tid; row < r1; row += kDecideThreads)
+  for (int row = r0 + tid; writes && row < r1; row += kThreads)
     if (row != stop) p.tokens_out[row] = row < stop ? p.tokens[row + 1] : -1;
+  __syncthreads();
+  return found;
 }
 
+// A sequence without rows, or with rows that are not there.
+__device__ __forceinline__ void no_rows(const VerifyParams& p, int b) {
+  if (threadIdx.x) return;
+  p.n_out[b] = 0;
+  p.drop[b] = 0;
+  if (p.cu_rows[b + 1] != p.cu_rows[b]) atomicExch(p.dev_err, kv4::kErrPage);
+}
+
+// One CTA per sequence.
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads) totals_kernel(const VerifyParams p) {
-  constexpr int N = Run<T>::N;
-  __shared__ double red[kStatThreads / 32], table[32];
-  fill_table(table);
+__global__ void __launch_bounds__(kDecideThreads) decide_kernel(const VerifyParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
-  const int r0 = first_row(p, b);
-  if (r0 < 0) return;
-  const Choice c = p.choice[r0];
-  if (c.row < 0) return;
-  const double inv_T = inverse_T(p, b);
-  __syncthreads();
-  const Chunk<T> chunk_of(p, c, chunk);
-  const Power ep(table, c.top, inv_T), eq(table, c.minus ? c.draft_top : 0.f, inv_T);
+  const int b = blockIdx.x, r0 = first_row(p, b);
+  if (r0 < 0) return no_rows(p, b);
+  const Choice c = decide<T, kDecideThreads>(p, b, r0, p.cu_rows[b + 1], true);
+  if (threadIdx.x == 0) p.choice[r0] = c;
+}
+
+// Sums of the exponentials of a chunk, the whole block's: target's (without a token that is left out) and draft's.
+template <typename T, int kThreads>
+__device__ __forceinline__ double2 totals_in(const Chunk<T>& chunk_of, const Choice& c, const Power& ep, const Power& eq, double* red) {
+  constexpr int N = Run<T>::N;
   double sp = 0.0, sq = 0.0;
-  for (int run = chunk_of.first + tid; run < chunk_of.end; run += 2 * kStatThreads) {
+  for (int run = chunk_of.first + (int)threadIdx.x; run < chunk_of.end; run += 2 * kThreads) {
     float a[2][N], d[2][N];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) chunk_of.load(run + h * kStatThreads, a[h], d[h]);
+    for (int h = 0; h < 2; ++h) chunk_of.load(run + h * kThreads, a[h], d[h]);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const double e = ep(a[h][i]);
         if (c.minus) sq += eq(d[h][i]);
-        if ((run + h * kStatThreads) * N + i != c.without) sp += e;
+        if ((run + h * kThreads) * N + i != c.without) sp += e;
       }
   }
-  sp = block_sum<kStatThreads>(sp, red);
-  if (c.minus) sq = block_sum<kStatThreads>(sq, red);
-  if (tid == 0) p.total[(int64_t)r0 * kMostChunks + chunk] = make_double2(sp, sq);
+  sp = block_sum<kThreads>(sp, red);
+  if (c.minus) sq = block_sum<kThreads>(sq, red);
+  return make_double2(sp, sq);
 }
 
-// sums over a sequence's chunks, by a whole warp
-__device__ __forceinline__ double2 totals_of(const VerifyParams& p, int r0) {
-  double sp = 0.0, sq = 0.0;
-  for (int k = threadIdx.x & 31; k < p.chunks; k += 32) {
-    const double2 v = p.total[(int64_t)r0 * kMostChunks + k];
-    sp += v.x;
-    sq += v.y;
-  }
-  return make_double2(warp_sum(sp), warp_sum(sq));
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kStatThreads) weights_kernel(const VerifyParams p) {
+// Sum of the weights max(p - q, 0) of a chunk.
+template <typename T, int kThreads>
+__device__ __forceinline__ double weights_in(const Chunk<T>& chunk_of, const Power& ep, const Power& eq, double ip, double iq, double* red) {
   constexpr int N = Run<T>::N;
-  __shared__ double red[kStatThreads / 32], table[32];
-  fill_table(table);
-  pdl_launch_dependents();
-  pdl_wait();
-  const int b = blockIdx.y, chunk = blockIdx.x;
-  const int r0 = first_row(p, b);
-  if (r0 < 0) return;
-  const Choice c = p.choice[r0];
-  if (c.row < 0 || !c.minus) return;         // else the totals are the weights' own
-  const Chunk<T> chunk_of(p, c, chunk);
-  const double inv_T = inverse_T(p, b);
-  const double2 total = totals_of(p, r0);
-  __syncthreads();
-  const Power ep(table, c.top, inv_T), eq(table, c.draft_top, inv_T);
-  const double ip = 1.0 / total.x, iq = 1.0 / total.y;
   double sum = 0.0;
-  for (int run = chunk_of.first + (int)threadIdx.x; run < chunk_of.end; run += kStatThreads) {
+  for (int run = chunk_of.first + (int)threadIdx.x; run < chunk_of.end; run += kThreads) {
     float a[N], d[N];
     double w[N];
     chunk_of.load(run, a, d);
@@ -485,43 +466,13 @@ __global__ void __launch_bounds__(kStatThreads) weights_kernel(const VerifyParam
 #pragma unroll
     for (int i = 0; i < N; ++i) sum += w[i];
   }
-  sum = block_sum<kStatThreads>(sum, red);
-  if (threadIdx.x == 0) p.weight[(int64_t)r0 * kMostChunks + chunk] = sum;
+  return block_sum<kThreads>(sum, red);
 }
 
-// One CTA per sequence: the chunk in which the running sum passes its goal, then the token.  By rounding there may be none; then the last with any weight.
-template <typename T>
-__global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyParams p) {
-  constexpr int kWarps = kChooseThreads / 32, N = Run<T>::N;
-  __shared__ double table[32], of_warp[kWarps];
-  __shared__ int token;
-  fill_table(table);
-  pdl_launch_dependents();
-  pdl_wait();
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r0 = first_row(p, b);
-  if (r0 < 0) return;
-  Choice c = p.choice[r0];
-  if (c.row < 0) return;
-  const double inv_T = inverse_T(p, b);
-  const double2 total = totals_of(p, r0);
-  // A lane has two neighbouring chunks.  p <= q everywhere, or nothing but the refused draft: the target itself.  (Where a token was left out, it is not in the totals.)
-  static_assert(kMostChunks == 64, "two chunks a lane");
-  double v0, v1, sum;
-  for (bool again = false;; again = true) {
-    auto at = [&](int k) { return k >= p.chunks ? 0.0 : c.minus ? p.weight[(int64_t)r0 * kMostChunks + k] : p.total[(int64_t)r0 * kMostChunks + k].x; };
-    v0 = at(2 * lane);
-    v1 = at(2 * lane + 1);
-    sum = warp_sum(v0 + v1);
-    if (sum > 0.0 || again || !c.minus) break;
-    c.minus = 0;
-  }
-  if (!(sum > 0.0)) {
-    if (tid == 0) p.tokens_out[c.row] = c.without;
-    return;
-  }
-  const double goal = (double)p.sample_u[b] * sum;
-  double before = v0 + v1;
+// Of up to 64 neighbouring sums, two per lane, the first at which the running sum passes the goal; by rounding there may be none, then the last above 0.  `before`: the sums in front of it.
+__device__ __forceinline__ int passing_part(double v0, double v1, double goal, double& before) {
+  const int lane = threadIdx.x & 31;
+  before = v0 + v1;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const double x = __shfl_up_sync(0xffffffffu, before, off);
@@ -530,16 +481,22 @@ __global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyPara
   const unsigned passing = __ballot_sync(0xffffffffu, v0 + v1 > 0.0 && before > goal), having = __ballot_sync(0xffffffffu, v0 + v1 > 0.0);
   const int who = passing ? __ffs(passing) - 1 : 31 - __clz(having);
   before -= v0 + v1;
-  int chunk = 2 * lane;
-  if (!(v0 > 0.0) || (v1 > 0.0 && !(before + v0 > goal))) { before += v0; ++chunk; }
-  chunk = __shfl_sync(0xffffffffu, chunk, who);
+  int part = 2 * lane;
+  if (!(v0 > 0.0) || (v1 > 0.0 && !(before + v0 > goal))) { before += v0; ++part; }
   before = __shfl_sync(0xffffffffu, before, who);
-  __syncthreads();                           // the table
-  const Chunk<T> chunk_of(p, c, chunk);
-  const Power ep(table, c.top, inv_T), eq(table, c.minus ? c.draft_top : 0.f, inv_T);
-  const double ip = 1.0 / total.x, iq = 1.0 / total.y;
+  return __shfl_sync(0xffffffffu, part, who);
+}
+
+// The token of a chunk at which the running sum, `before` in front of the chunk, passes the goal, or the last with any weight.
+template <typename T, int kThreads>
+__device__ __forceinline__ void find_token(const VerifyParams& p, const Chunk<T>& chunk_of, const Choice& c, const Power& ep, const Power& eq, double ip, double iq, double before,
+                                           double goal) {
+  constexpr int kWarps = kThreads / 32, N = Run<T>::N;
+  __shared__ double of_warp[kWarps];
+  __shared__ int token, first_pass, last_some;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) token = -1;
-  for (int base = chunk_of.first; base < chunk_of.end; base += kChooseThreads) {
+  for (int base = chunk_of.first; base < chunk_of.end; base += kThreads) {
     const int run = base + tid;
     float a[N], d[N];
     double w[N], v = 0.0;
@@ -561,7 +518,6 @@ __global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyPara
     for (int k = 0; k < kWarps; ++k) before += of_warp[k];
     // the first run that passes has the token; without one the last run with any weight, so far
     const bool passes = v > 0.0 && mine + v > goal;
-    __shared__ int first_pass, last_some;
     if (tid == 0) { first_pass = INT_MAX; last_some = -1; }
     __syncthreads();
     if (passes) atomicMin(&first_pass, run);
@@ -582,9 +538,155 @@ __global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyPara
 }
 
 template <typename T>
+__global__ void __launch_bounds__(kStatThreads) totals_kernel(const VerifyParams p) {
+  __shared__ double red[kStatThreads / 32], table[32];
+  fill_table(table);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
+  const int r0 = first_row(p, b);
+  if (r0 < 0) return;
+  const Choice c = p.choice[r0];
+  if (c.row < 0) return;
+  const double inv_T = inverse_T(p, b);
+  __syncthreads();
+  const double2 t = totals_in<T, kStatThreads>(Chunk<T>(p, c, chunk), c, Power(table, c.top, inv_T), Power(table, c.minus ? c.draft_top : 0.f, inv_T), red);
+  if (tid == 0) p.total[(int64_t)r0 * kMostChunks + chunk] = t;
+}
+
+// sums over a sequence's chunks, by a whole warp
+__device__ __forceinline__ double2 totals_of(const VerifyParams& p, int r0) {
+  double sp = 0.0, sq = 0.0;
+  for (int k = threadIdx.x & 31; k < p.chunks; k += 32) {
+    const double2 v = p.total[(int64_t)r0 * kMostChunks + k];
+    sp += v.x;
+    sq += v.y;
+  }
+  return make_double2(warp_sum(sp), warp_sum(sq));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kStatThreads) weights_kernel(const VerifyParams p) {
+  __shared__ double red[kStatThreads / 32], table[32];
+  fill_table(table);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.y, chunk = blockIdx.x;
+  const int r0 = first_row(p, b);
+  if (r0 < 0) return;
+  const Choice c = p.choice[r0];
+  if (c.row < 0 || !c.minus) return;         // else the totals are the weights' own
+  const double inv_T = inverse_T(p, b);
+  const double2 total = totals_of(p, r0);
+  __syncthreads();
+  const double w = weights_in<T, kStatThreads>(Chunk<T>(p, c, chunk), Power(table, c.top, inv_T), Power(table, c.draft_top, inv_T), 1.0 / total.x, 1.0 / total.y, red);
+  if (threadIdx.x == 0) p.weight[(int64_t)r0 * kMostChunks + chunk] = w;
+}
+
+// One CTA per sequence: the chunk in which the running sum passes its goal, then the token.
+template <typename T>
+__global__ void __launch_bounds__(kChooseThreads) choose_kernel(const VerifyParams p) {
+  __shared__ double table[32];
+  fill_table(table);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x, lane = threadIdx.x & 31;
+  const int r0 = first_row(p, b);
+  if (r0 < 0) return;
+  Choice c = p.choice[r0];
+  if (c.row < 0) return;
+  const double inv_T = inverse_T(p, b);
+  const double2 total = totals_of(p, r0);
+  static_assert(kMostChunks == 64, "two chunks a lane");
+  double v0, v1, sum;
+  for (bool again = false;; again = true) {  // p <= q everywhere: the target itself
+    auto at = [&](int k) { return k >= p.chunks ? 0.0 : c.minus ? p.weight[(int64_t)r0 * kMostChunks + k] : p.total[(int64_t)r0 * kMostChunks + k].x; };
+    v0 = at(2 * lane);
+    v1 = at(2 * lane + 1);
+    sum = warp_sum(v0 + v1);
+    if (sum > 0.0 || again || !c.minus) break;
+    c.minus = 0;
+  }
+  if (!(sum > 0.0)) {                        // nothing but the refused draft
+    if (threadIdx.x == 0) p.tokens_out[c.row] = c.without;
+    return;
+  }
+  const double goal = (double)p.sample_u[b] * sum;
+  double before;
+  const int chunk = passing_part(v0, v1, goal, before);
+  __syncthreads();                           // the table
+  find_token<T, kChooseThreads>(p, Chunk<T>(p, c, chunk), c, Power(table, c.top, inv_T), Power(table, c.minus ? c.draft_top : 0.f, inv_T), 1.0 / total.x, 1.0 / total.y, before, goal);
+}
+
+// All of that in one launch, a cluster per sequence and a CTA per chunk: where there is little to do, the launches are what it takes.
+template <typename T>
+__global__ void __launch_bounds__(kChooseThreads) at_once_kernel(const VerifyParams p) {
+  namespace cg = cooperative_groups;
+  __shared__ double red[kChooseThreads / 32], table[32], mine[4];        // this CTA's sums, read by its cluster
+  fill_table(table);
+  pdl_launch_dependents();
+  pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31;
+  const int r0 = first_row(p, b);
+  if (r0 < 0) {                              // the same for the whole cluster, as every return before its last barrier
+    if (rank == 0) no_rows(p, b);
+    return;
+  }
+  Choice c = decide<T, kChooseThreads>(p, b, r0, p.cu_rows[b + 1], rank == 0);
+  if (c.row < 0) return;
+  const double inv_T = inverse_T(p, b);
+  const Chunk<T> chunk_of(p, c, rank);
+  const Power ep(table, c.top, inv_T), eq(table, c.minus ? c.draft_top : 0.f, inv_T);
+  const double2 t = totals_in<T, kChooseThreads>(chunk_of, c, ep, eq, red);
+  if (tid == 0) { mine[0] = t.x; mine[1] = t.y; }
+  cluster.sync();
+  auto of = [&](int what, int k) { return k < C ? *cluster.map_shared_rank(mine + what, k) : 0.0; };
+  const double sp = warp_sum(of(0, lane)), sq = warp_sum(of(1, lane));
+  const double ip = 1.0 / sp, iq = 1.0 / sq;
+  double v0 = of(0, 2 * lane), v1 = of(0, 2 * lane + 1), sum = sp;
+  if (c.minus) {
+    const double w = weights_in<T, kChooseThreads>(chunk_of, ep, eq, ip, iq, red);
+    if (tid == 0) mine[2] = w;
+    cluster.sync();
+    const double s = warp_sum(of(2, lane));
+    if (s > 0.0) { sum = s; v0 = of(2, 2 * lane); v1 = of(2, 2 * lane + 1); }
+    else c.minus = 0;                        // p <= q everywhere: the target itself
+  }
+  cluster.sync();                            // no CTA leaves while others read its sums
+  if (!(sum > 0.0)) {                        // nothing but the refused draft
+    if (rank == 0 && tid == 0) p.tokens_out[c.row] = c.without;
+    return;
+  }
+  const double goal = (double)p.sample_u[b] * sum;
+  double before;
+  if (passing_part(v0, v1, goal, before) != rank) return;
+  find_token<T, kChooseThreads>(p, Chunk<T>(p, c, rank), c, ep, eq, ip, iq, before, goal);
+}
+
+template <typename T>
 int32_t launch_verify(Ctx* ctx, const VerifyParams& p) {
   LMB_CUDA(launch_k_opt(false, statistics_kernel<T>, dim3((unsigned)p.splits, (unsigned)p.rows), dim3(kStatThreads), 0, ctx->stream, p));
   ctx->launches++;
+  if (p.vocab <= kAtOnce) {
+    VerifyParams q = p;
+    q.chunks = p.vocab <= 4096 ? 1 : 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(q.n_seq * q.chunks));
+    cfg.blockDim = dim3(kChooseThreads);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)q.chunks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    LMB_CUDA(cudaLaunchKernelEx(&cfg, at_once_kernel<T>, q));
+    ctx->launches++;
+    return LMB200_OK;
+  }
   const dim3 grid((unsigned)p.chunks, (unsigned)p.n_seq);
   LMB_CUDA(launch_k(decide_kernel<T>, dim3((unsigned)p.n_seq), dim3(kDecideThreads), 0, ctx->stream, p));
   ctx->launches++;
