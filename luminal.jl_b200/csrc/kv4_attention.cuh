@@ -10,7 +10,7 @@
 // step has 1 to 8 of them: on tcgen05 M would be padded to 128, and the 4-bit operand would have to be widened through shared memory instead of in registers.
 //
 // Work.  Units of 128 keys of all (sequence, row tile, kv head) triples in a row are cut into equal shares whatever the sequences' lengths, so a long sequence among short ones
-// is shared by many CTAs.  Each of a CTA's four warps takes 32 keys of a unit through a ring of bulk copies of its own, which is filled with the next triple's keys while the present
+// is shared by many CTAs.  Little work is cut into pieces of triples instead, one per CTA, if none becomes much longer than a share: a second triple costs a CTA about 7 us.  Each of a CTA's four warps takes 32 keys of a unit through a ring of bulk copies of its own, which is filled with the next triple's keys while the present
 // one's sums are joined.  Where a triple is cut, its shares leave partial sums and the last one to finish joins them (many: in groups first).
 #pragma once
 #include <math_constants.h>
@@ -24,6 +24,7 @@ namespace kv4 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kUnit = 128, kMaxSeqs = 8192;
 constexpr int kCounters = 4096, kMostShares = kCounters / 2, kJoin = 16;
+constexpr unsigned kLonger = 8;                // units by which a piece may be longer than a share
 
 struct Params {
   const void* q;
@@ -102,6 +103,8 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+// all ones in the halves that are infinite or no number
+__device__ __forceinline__ uint32_t odd_halves(uint32_t u) { return __vcmpgtu2(u & 0x7fff7fffu, 0x7bff7bffu); }
 // two of a word's numbers as MMA operand: n 2^-24 (16 n 2^-24 for the high ones), or, normal, n (16 n)
 template <bool kNormal> __device__ __forceinline__ uint32_t numbers(uint32_t x, uint32_t mask) {
   x &= mask;
@@ -114,17 +117,18 @@ __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast
 // What a warp works on, and where it stands in its CTA's share: in shared memory, because the pass over the keys has no registers to spare.  The warps of a CTA all write the
 // same segment, into one of three places in turn.
 struct Segment {
-  int64_t item0;                             // the triple's first unit in the common order
+  int64_t item0;                             // the triple's first piece in the common order
   const int* row_table;
   const uint8_t* head_pages;                 // of its kv head in page 0
   int tile, head, valid, pad;                // valid: query rows of the tile
   int rows0, position0;                      // of the sequence's first new token
-  int n_units, from_unit, to_unit;           // of the triple: units [from_unit, to_unit)
+  int n_pieces, from_piece, to_piece;        // of the triple: pieces [from_piece, to_piece)
+  int n_stages;                              // units of those
   int first_block, highest, lowest;          // keys that some row sees
   int all_from, all_to;                      // keys that all rows see
 };
 struct Walk {
-  int64_t u;                                 // first unit that is left of the share
+  int64_t u;                                 // first piece that is left of the share
   int b, pad;                                // its sequence
 };
 
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
   int* shared_word = reinterpret_cast<int*>(at); at += 64;  // 0..3 sums of warps, 4 the last one's flag
   Segment* segments = reinterpret_cast<Segment*>(at); at += 3 * 96;
   Walk* walk = reinterpret_cast<Walk*>(at) + (threadIdx.x >> 5); at += kWarps * 16;
-  unsigned* before = reinterpret_cast<unsigned*>(at);      // [n_seq + 1] units of the sequences before
+  unsigned* before = reinterpret_cast<unsigned*>(at);      // [n_seq + 1] pieces of the sequences before
   int* seq_len = reinterpret_cast<int*>(before + p.n_seq + 1);           // [n_seq] their tokens
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -164,7 +168,8 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
   pdl_launch_dependents();
   pdl_wait();
 
-  // units of every sequence
+  // pieces of every sequence
+  unsigned piece = 1;
   auto units_of = [&](int T_, int len, int& first) __attribute__((always_inline)) {
     const int lowest = len - T_;                           // position of the first row
     first = p.window > 0 && lowest - p.window + 1 > 0 ? (lowest - p.window + 1) / kUnit : 0;
@@ -174,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
     const int capacity = p.max_pages << p.shift;
     const int per = (p.n_seq + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, p.n_seq), b1 = min(b0 + per, p.n_seq);
-    unsigned sum = 0;
+    unsigned sum = 0, items = 0;
     bool bad = false;
     for (int b = b0; b < b1; ++b) {
       const int r0 = p.cu_rows[b], r1 = p.cu_rows[b + 1], l = p.lens[b];
@@ -182,27 +187,56 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
       int T_ = r1 - r0, first;
       bad |= l != len;
       if (r0 < 0 || r1 < r0 || r1 > p.rows) { bad = true; T_ = 0; }
-      const unsigned n = T_ > 0 ? (unsigned)row_tiles(T_, p.G, COLS) * p.heads * units_of(T_, len, first) : 0u;
+      const unsigned triples = T_ > 0 ? (unsigned)row_tiles(T_, p.G, COLS) * p.heads : 0u, n = triples * units_of(T_, len, first);
       seq_len[b] = len;
       before[b + 1] = n;
       sum += n;
+      items += triples;
     }
     if (bad && blockIdx.x == 0) atomicExch(p.dev_err, kErrPage);
+    // units per piece: 1, or so many that every CTA has one piece
+    {
+      unsigned all = sum, of = items;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, off);
+        of += __shfl_xor_sync(0xffffffffu, of, off);
+      }
+      if (lane == 0) { shared_word[warp] = (int)all; shared_word[8 + warp] = (int)of; }
+      __syncthreads();
+      all = of = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) { all += (unsigned)shared_word[w]; of += (unsigned)shared_word[8 + w]; }
+      if (of < gridDim.x) {
+        const unsigned room = gridDim.x - of, each = (all + room - 1) / room;            // sum of ceil(n / each) <= all / each + of <= the CTAs
+        if (each <= all / gridDim.x + kLonger) piece = max(1u, each);
+      }
+    }
+    if (piece > 1) {
+      sum = 0;
+      for (int b = b0; b < b1; ++b) {
+        if (before[b + 1] == 0) continue;
+        int first;
+        const int T_ = p.cu_rows[b + 1] - p.cu_rows[b];
+        before[b + 1] = (unsigned)row_tiles(T_, p.G, COLS) * p.heads * ((units_of(T_, seq_len[b], first) + piece - 1) / piece);
+        sum += before[b + 1];
+      }
+    }
     unsigned incl = sum;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const unsigned u = __shfl_up_sync(0xffffffffu, incl, off);
       if (lane >= off) incl += u;
     }
-    if (lane == 31) shared_word[warp] = (int)incl;
+    if (lane == 31) shared_word[4 + warp] = (int)incl;
     __syncthreads();
     unsigned run = incl - sum;
-    for (int w = 0; w < warp; ++w) run += (unsigned)shared_word[w];
+    for (int w = 0; w < warp; ++w) run += (unsigned)shared_word[4 + w];
     for (int b = b0; b < b1; ++b) { run += before[b + 1]; before[b + 1] = run; }
     if (tid == 0) before[0] = 0;
     __syncthreads();
   }
-  // every CTA that takes part has a share, every share a unit
+  // every CTA that takes part has a share, every share a piece
   const int64_t U = before[p.n_seq];
   const int grid = (int)min((int64_t)gridDim.x, U);
   if ((int)blockIdx.x >= grid) return;
@@ -219,11 +253,13 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
     int first_unit;
     const int rows0 = p.cu_rows[b], T_ = p.cu_rows[b + 1] - rows0, len = seq_len[b];
     const int n_units = units_of(T_, len, first_unit);
-    const int triple = (int)(u - before[b]) / n_units, tile = triple / p.heads, head = triple - tile * p.heads;
-    const int64_t item0 = (int64_t)before[b] + (int64_t)triple * n_units;
+    const int n_pieces = (n_units + (int)piece - 1) / (int)piece;        // of as equal lengths as units allow
+    const int triple = (int)(u - before[b]) / n_pieces, tile = triple / p.heads, head = triple - tile * p.heads;
+    const int64_t item0 = (int64_t)before[b] + (int64_t)triple * n_pieces;
     const int valid = min(COLS, T_ * p.G - tile * COLS);                 // query rows of this tile; their positions ascend
     const int first_pos = len - T_ + tile * COLS / p.G, last_pos = len - T_ + (tile * COLS + valid - 1) / p.G;
-    const int to_unit = (int)min((int64_t)n_units, u_end - item0);
+    const int from_piece = (int)(u - item0), to_piece = (int)min((int64_t)n_pieces, u_end - item0);
+    const int from_unit = (int)((int64_t)n_units * from_piece / n_pieces), to_unit = (int)((int64_t)n_units * to_piece / n_pieces);
     __syncwarp();
     if (lane == 0) {
       sg->item0 = item0;
@@ -231,13 +267,14 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
       sg->head_pages = p.pages + (int64_t)head * per_page * (640 * NG);
       sg->tile = tile; sg->head = head; sg->valid = valid;
       sg->rows0 = rows0; sg->position0 = len - T_;
-      sg->n_units = n_units; sg->from_unit = (int)(u - item0); sg->to_unit = to_unit;
-      sg->first_block = (first_unit + (int)(u - item0)) * (kUnit / 16);
+      sg->n_pieces = n_pieces; sg->from_piece = from_piece; sg->to_piece = to_piece;
+      sg->n_stages = to_unit - from_unit;
+      sg->first_block = (first_unit + from_unit) * (kUnit / 16);
       sg->highest = max(0, last_pos + 1);
       sg->lowest = p.window > 0 ? max(0, first_pos - p.window + 1) : 0;
       sg->all_from = p.window > 0 ? max(0, last_pos - p.window + 1) : 0;
       sg->all_to = max(0, first_pos + 1);
-      walk->u = item0 + to_unit; walk->b = b;
+      walk->u = item0 + to_piece; walk->b = b;
     }
     __syncwarp();
     return true;
@@ -249,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
   bool dead = false;
   auto place_of = [&](const Segment* sg, int batch) __attribute__((always_inline)) {       // lane: block lane % 2 of stage 16 batch + lane / 2; -1: not to be read
     const int j = batch * 16 + (lane >> 1), key = (sg->first_block + 2 * warp + j * (kUnit / 16) + (lane & 1)) * 16;
-    return j < sg->to_unit - sg->from_unit && key < sg->highest && key + 16 > sg->lowest ? key >> p.shift : -1;
+    return j < sg->n_stages && key < sg->highest && key + 16 > sg->lowest ? key >> p.shift : -1;
   };
   auto page_at = [&](const Segment* sg, int batch) __attribute__((always_inline)) {
     const int place = place_of(sg, batch);
@@ -287,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
     ids = checked(sg, 0, page0);
     ids_next = page1;
     slot = 0;
-    const int n = min(kStages, sg->to_unit - sg->from_unit);
+    const int n = min(kStages, sg->n_stages);
 #pragma unroll 1
     for (int s = 0; s < n; ++s) issue(sg, s, s);
   };
@@ -341,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
   auto count_part = [&](const Segment* my) __attribute__((always_inline)) {
     Part q;
     q.sa = (int)(((my->item0 + 1) * grid - 1) / U);
-    const int n = (int)(((my->item0 + my->n_units) * grid - 1) / U) - q.sa + 1;
+    const int n = (int)(((my->item0 + my->n_pieces) * grid - 1) / U) - q.sa + 1;
     const bool grouped = n > kJoin + kJoin / 2;
     const int group = grouped ? ((int)blockIdx.x - q.sa) / kJoin : 0;
     q.groups = grouped ? (n + kJoin - 1) / kJoin : 1;
@@ -491,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
     float m[NT][2], l[NT][2], o[2 * NG][NT][4], om[NT][4];
     int r;
     uint32_t seen;                           // columns that have a maximum; m of the others is 0
-    const int n_stages = sg->to_unit - sg->from_unit, first_key = (sg->first_block + 2 * warp) * 16, all_from = sg->all_from, all_to = sg->all_to;
+    const int n_stages = sg->n_stages, first_key = (sg->first_block + 2 * warp) * 16, all_from = sg->all_from, all_to = sg->all_to;
     for (bool careful = false;; careful = true) {
     r = 0;
     seen = 0;
@@ -514,8 +551,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
         tc::mbar_wait(my_full + slot, phases >> slot & 1u, dead, p.dev_err);
         phases ^= 1u << slot;
         const int key0 = first_key + j * kUnit;
-        // a stage that all rows see whole, once they all have a maximum, needs nothing looked at
-        const bool look = bits != 3u || key0 < all_from || key0 + 32 > all_to || !ready || careful;
+        const bool cut = bits != 3u || key0 < all_from || key0 + 32 > all_to;              // some row does not see all of it
         const uint8_t* stage0 = my_ring + slot * S::kStageBytes;
 #pragma unroll 1
         for (int k0 = 0; k0 < 2; k0 += BK) {
@@ -612,9 +648,9 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
               }
               raise |= top > kPScale + 8.f;
             }
-          if (look || __any_sync(0xffffffffu, raise)) {
-            if (look) {
-              __half2 most = __float2half2_rn(0.f);
+          bool odd_values = false;           // a scale or minimum of a value that is no number
+          if (cut || careful || !ready || __any_sync(0xffffffffu, raise)) {
+            if (cut) {
 #pragma unroll
               for (int kb = 0; kb < BK; ++kb) {
                 const bool there = bits >> (k0 + kb) & 1;
@@ -625,20 +661,35 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                     const int key = key0 + (k0 + kb) * 16 + g + (k >= 2 ? 8 : 0), c = nt * 8 + 2 * t + (k & 1);
                     if (key >= col_end[c] || key < col_from[c] || !there) s[kb][nt][k] = -CUDART_INF_F;
                   }
-                // A key's value that is no number counts for the rows that see the key alone: a minimum that is none makes its scale one, and scales meet weights below.
-                // A key that no row sees counts for none.
                 if (!there) mn[kb] = make_uint2(0, 0);
-                const uint32_t ox = __vcmpgtu2(mn[kb].x & 0x7fff7fffu, 0x7bff7bffu), oy = __vcmpgtu2(mn[kb].y & 0x7fff7fffu, 0x7bff7bffu);
-                mn[kb].x &= ~ox;
-                mn[kb].y &= ~oy;
+                uint32_t odd = odd_halves(mn[kb].x) | odd_halves(mn[kb].y);
 #pragma unroll
                 for (int gr = 0; gr < NG; ++gr) {
                   if (!there) vs[kb][gr] = make_uint2(0, 0);
-                  most = __hmax2(most, __hmax2(as_half2(vs[kb][gr].x), as_half2(vs[kb][gr].y)));
-                  vs[kb][gr].x |= __shfl_sync(0xffffffffu, ox, gr * 4 + t) & 0x7fff7fffu;
-                  vs[kb][gr].y |= __shfl_sync(0xffffffffu, oy, gr * 4 + t) & 0x7fff7fffu;
+                  odd |= odd_halves(vs[kb][gr].x) | odd_halves(vs[kb][gr].y);
+                }
+                odd_values |= odd != 0;
+              }
+              odd_values = __any_sync(0xffffffffu, odd_values);
+              if (odd_values) {              // they take no part here; below, the rows that see them get them
+#pragma unroll
+                for (int kb = 0; kb < BK; ++kb) {
+                  mn[kb].x &= ~odd_halves(mn[kb].x);
+                  mn[kb].y &= ~odd_halves(mn[kb].y);
+#pragma unroll
+                  for (int gr = 0; gr < NG; ++gr) {
+                    vs[kb][gr].x &= ~odd_halves(vs[kb][gr].x);
+                    vs[kb][gr].y &= ~odd_halves(vs[kb][gr].y);
+                  }
                 }
               }
+            }
+            if (careful) {
+              __half2 most = __float2half2_rn(0.f);
+#pragma unroll
+              for (int kb = 0; kb < BK; ++kb)
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) most = __hmax2(most, __hmax2(as_half2(vs[kb][gr].x), as_half2(vs[kb][gr].y)));
               float x = fmaxf(__low2float(most), __high2float(most));
 #pragma unroll
               for (int off = 1; off < 4; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
@@ -675,20 +726,21 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                 const float rise = x - kPScale;
                 const bool first = !(seen >> (2 * nt + k) & 1);
                 if (first ? x > -CUDART_INF_F : rise > 0.f) {
-                  const float fade = first ? 0.f : exp2_fast(-rise);
                   seen |= 1u << (2 * nt + k);
                   m[nt][k] += rise;
-                  l[nt][k] *= fade;
-                  om[nt][k] *= fade;
-                  om[nt][k + 2] *= fade;
+                  if (!first) {
+                    const float fade = exp2_fast(-rise);
+                    l[nt][k] *= fade;
+                    om[nt][k] *= fade;
+                    om[nt][k + 2] *= fade;
 #pragma unroll
-                  for (int i = 0; i < 2 * NG; ++i) { o[i][nt][k] *= fade; o[i][nt][k + 2] *= fade; }
+                    for (int i = 0; i < 2 * NG; ++i) { o[i][nt][k] *= fade; o[i][nt][k + 2] *= fade; }
+                  }
 #pragma unroll
                   for (int kb = 0; kb < BK; ++kb) { s[kb][nt][k] -= rise; s[kb][nt][k + 2] -= rise; }
                 }
               }
-            // (larger scales keep the quick way closed)
-            ready = r == 0 && __all_sync(0xffffffffu, seen == (1u << (2 * NT)) - 1u);
+            ready = __all_sync(0xffffffffu, seen == (1u << (2 * NT)) - 1u);
           }
           // weights as halves (float32: two of them), from accumulators to B operands; then values
 #pragma unroll
@@ -712,6 +764,21 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
               if (kSplit) mma_split<false>(om[nt], mn[kb].x, 0u, mn[kb].y, 0u, pb[nt][0], pb[nt][1], pb[nt][kSplit ? 2 : 0], pb[nt][kSplit ? 3 : 0]);
               else mma_half(om[nt], mn[kb].x, 0u, mn[kb].y, 0u, pb[nt][0], pb[nt][1]);
             }
+            if (odd_values && (bits >> (k0 + kb) & 1)) {
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr) {
+                const uint8_t* block = stage + kb * 640 * NG;
+                const uint2 sc = *reinterpret_cast<const uint2*>(block + 576 * NG + gr * 32 + t * 8), mi = *reinterpret_cast<const uint2*>(block + 608 * NG + gr * 32 + t * 8);
+                const uint32_t ox = odd_halves(sc.x) | odd_halves(mi.x), oy = odd_halves(sc.y) | odd_halves(mi.y);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {            // lane (g, t): row g's weights of keys 2t, 2t + 1, 2t + 8, 2t + 9
+                  const unsigned hit = __ballot_sync(0xffffffffu, (pb[nt][0] & ox) | (pb[nt][1] & oy));
+#pragma unroll
+                  for (int k = 0; k < 2; ++k)
+                    if (hit >> (4 * (2 * t + k)) & 15) o[2 * gr][nt][k] = o[2 * gr][nt][k + 2] = o[2 * gr + 1][nt][k] = o[2 * gr + 1][nt][k + 2] = CUDART_NAN_F;
+                }
+              }
+            }
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
               const uint2 w = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 256 * NG + gr * 256 + lane * 8);
@@ -723,11 +790,7 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
 #pragma unroll
                   for (int i = 0; i < 2; ++i) {
                     const float2 hi = __half22float2(as_half2(pb[nt][i])), lo = __half22float2(as_half2(pb[nt][kSplit ? 2 + i : 0]));
-                    float x = (hi.x + lo.x) * (i ? sy.x : sx.x), y = (hi.y + lo.y) * (i ? sy.y : sx.y);
-                    if (look) {
-                      if (hi.x == 0.f) x = 0.f;
-                      if (hi.y == 0.f) y = 0.f;
-                    }
+                    const float x = (hi.x + lo.x) * (i ? sy.x : sx.x), y = (hi.y + lo.y) * (i ? sy.y : sx.y);
                     wb[nt][i] = pack(x, y);
                     const float2 f = __half22float2(as_half2(wb[nt][i]));
                     wb[nt][kSplit ? 2 + i : 0] = pack(x - f.x, y - f.y);
@@ -735,13 +798,6 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                 } else {
                   wb[nt][0] = as_u32(__hmul2(as_half2(pb[nt][0]), as_half2(vs[kb][gr].x)));
                   wb[nt][1] = as_u32(__hmul2(as_half2(pb[nt][1]), as_half2(vs[kb][gr].y)));
-                }
-              }
-              if (!kSplit && look) {         // a weight of 0 takes no part
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  wb[nt][0] &= __vcmpne2(pb[nt][0], 0u);
-                  wb[nt][1] &= __vcmpne2(pb[nt][1], 0u);
                 }
               }
 #pragma unroll
@@ -830,8 +886,8 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
       }
       __syncthreads();
     }
-    const bool alone = sg->from_unit == 0 && sg->to_unit == sg->n_units;
-    const int part = (int)blockIdx.x * 2 + (sg->from_unit == 0 ? 1 : 0);
+    const bool alone = sg->from_piece == 0 && sg->to_piece == sg->n_pieces;
+    const int part = (int)blockIdx.x * 2 + (sg->from_piece == 0 ? 1 : 0);
     for (int i = tid; i < sg->valid * (D / 4); i += kThreads) {
       const int c = i / (D / 4), d = (i - c * (D / 4)) * 4;
       float top = -CUDART_INF_F, L = 0.f;
