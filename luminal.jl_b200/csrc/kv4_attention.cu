@@ -12,7 +12,7 @@ int grid_of(const Ctx* ctx, const kv4::Variant* v) { return std::min(ctx->sm_cou
 int64_t workspace_bytes_of(const Ctx* ctx, int D) {
   int64_t most = 0;
   for (int f32 = 0; f32 < 2; ++f32)
-    for (int nt = 1; nt <= kv4::most_tiles(f32, kv4::groups(D)); ++nt)
+    for (int nt = 1; nt <= kv4::kMostTiles; ++nt)
       most = std::max<int64_t>(most, (int64_t)grid_of(ctx, f32 ? kv4::variant_f32(kv4::groups(D), nt) : kv4::variant_bf16(kv4::groups(D), nt)) * 2 * (8 * nt) * (D + 2) * 4);
   return kv4::kCounters * 4 + most;
 }
@@ -58,11 +58,13 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   const int64_t need = workspace_bytes_of(ctx, head_dim);
   LMB_REQUIRE(workspace_bytes >= need, "kv4_attention: a workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
   if (rows == 0) return LMB200_OK;
-  // Query rows of one kv head that share a pass over its keys, in tiles of 8: what a sequence has on average (only the device knows each one's), as far as registers go.
+  // Query rows of one kv head that share a pass over its keys: 8, or 16 where that makes 3/5 as many passes or fewer (a pass for 16 takes 5/3 of one for 8).  Only the device knows
+  // how many rows each sequence has; the average decides.  24 rows (6 drafts of 4 heads): 66 us as three eights, 74 as two sixteens; 16 rows: 44 and 42; 1024: 345 and 268.  Tiles of 24
+  // and 32 rows leave registers for two CTAs an SM and were slower everywhere (71 and 92 us for the 24 rows).
   const bool f32 = dtype == LMB200_F32;
   const int NG = kv4::groups(head_dim);
-  const int64_t each = ceil_div(ceil_div(rows, n_seq) * group, 8);
-  const int NT = (int)std::min<int64_t>(each, kv4::most_tiles(f32, NG));
+  const int64_t each = ceil_div(rows, n_seq) * group;
+  const int NT = ceil_div(each, 16) * 5 <= ceil_div(each, 8) * 3 ? 2 : 1;
   const kv4::Variant* v = f32 ? kv4::variant_f32(NG, NT) : kv4::variant_bf16(NG, NT);
   // units of work are counted in 32 bits
   const int64_t tiles = ceil_div((int64_t)rows * group, 8 * NT) + std::min(n_seq, rows), units = ceil_div((int64_t)max_pages * page_size, kv4::kUnit) + 1;

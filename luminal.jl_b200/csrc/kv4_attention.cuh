@@ -24,7 +24,7 @@ namespace kv4 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kUnit = 128, kMaxSeqs = 8192;
 constexpr int kCounters = 4096, kMostShares = kCounters / 2, kJoin = 16;
-constexpr unsigned kLonger = 8;                // units by which a piece may be longer than a share
+constexpr unsigned kLonger = 8;                    // units by which a piece may be longer than a share
 
 struct Params {
   const void* q;
@@ -52,14 +52,13 @@ const Variant* variant_bf16(int NG, int NT);
 const Variant* variant_f32(int NG, int NT);
 int32_t configure_bf16();
 int32_t configure_f32();
-// most query rows that share a pass over the keys, in tiles of 8: what the registers hold of out (8 NG values of it per tile and thread)
-__host__ __device__ constexpr int most_tiles(bool f32, int NG) { return f32 ? 2 : NG <= 4 ? 4 : 2; }
+constexpr int kMostTiles = 2;
 
 template <typename T, int NG, int NT> struct Shape {
   static constexpr bool kSplit = sizeof(T) == 4;          // float32: operands as two halves, 22 bits
   static constexpr int D = 32 * NG, COLS = 8 * NT;
   static constexpr int kStageBytes = 2 * 640 * NG;
-  static constexpr int kStages = NG == 1 ? 8 : NG == 2 ? 6 : NG == 3 ? 4 : NG <= 5 ? 3 : 2;
+  static constexpr int kStages = NG == 1 ? 8 : NG == 2 ? 4 : NG == 3 ? 3 : 2;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kPitch = D + 4;                    // of the joined sums: 2 kPitch = 8 banks
   static constexpr int kMerge = 2 * COLS * kPitch * 4;
@@ -135,11 +134,11 @@ struct Walk {
 __device__ __forceinline__ int row_tiles(int T, int G, int cols) { return (T * G + cols - 1) / cols; }
 
 template <typename T, int NG, int NT>
-__global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attention_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) attention_kernel(const Params p) {
   using S = Shape<T, NG, NT>;
   constexpr int D = S::D, COLS = S::COLS, kStages = S::kStages;
   constexpr bool kSplit = S::kSplit;
-  constexpr int BK = NT <= 2 ? 2 : 1;        // blocks of 16 keys whose scores are in registers at once
+  constexpr int BK = 2;                      // blocks of 16 keys whose scores are in registers at once
   constexpr float kPScale = 7.f;             // weights are 2^7 p at the maximum, up to 2^15 while it lags
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* at = smem;
@@ -208,18 +207,26 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) { all += (unsigned)shared_word[w]; of += (unsigned)shared_word[8 + w]; }
       if (of < gridDim.x) {
-        const unsigned room = gridDim.x - of, each = (all + room - 1) / room;            // sum of ceil(n / each) <= all / each + of <= the CTAs
-        if (each <= all / gridDim.x + kLonger) piece = max(1u, each);
-      }
-    }
-    if (piece > 1) {
-      sum = 0;
-      for (int b = b0; b < b1; ++b) {
-        if (before[b + 1] == 0) continue;
-        int first;
-        const int T_ = p.cu_rows[b + 1] - p.cu_rows[b];
-        before[b + 1] = (unsigned)row_tiles(T_, p.G, COLS) * p.heads * ((units_of(T_, seq_len[b], first) + piece - 1) / piece);
-        sum += before[b + 1];
+        const unsigned room = gridDim.x - of, each = max(1u, (all + room - 1) / room);           // sum of ceil(n / each) <= all / each + of <= the CTAs
+        unsigned longest = 0, pieces = 0;
+        for (int b = b0; b < b1; ++b) {
+          if (before[b + 1] == 0) continue;
+          int first;
+          const int T_ = p.cu_rows[b + 1] - p.cu_rows[b];
+          const unsigned n = units_of(T_, seq_len[b], first), k = (n + each - 1) / each;
+          longest = max(longest, (n + k - 1) / k);
+          pieces += (unsigned)row_tiles(T_, p.G, COLS) * p.heads * k;
+        }
+        if (!__syncthreads_or(longest > all / gridDim.x + kLonger)) {
+          piece = each;
+          sum = pieces;
+          for (int b = b0; b < b1; ++b) {
+            if (before[b + 1] == 0) continue;
+            int first;
+            const int T_ = p.cu_rows[b + 1] - p.cu_rows[b];
+            before[b + 1] = (unsigned)row_tiles(T_, p.G, COLS) * p.heads * ((units_of(T_, seq_len[b], first) + each - 1) / each);
+          }
+        }
       }
     }
     unsigned incl = sum;
@@ -552,10 +559,8 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
         phases ^= 1u << slot;
         const int key0 = first_key + j * kUnit;
         const bool cut = bits != 3u || key0 < all_from || key0 + 32 > all_to;              // some row does not see all of it
-        const uint8_t* stage0 = my_ring + slot * S::kStageBytes;
-#pragma unroll 1
-        for (int k0 = 0; k0 < 2; k0 += BK) {
-          const uint8_t* stage = stage0 + k0 * 640 * NG;
+        const uint8_t* stage = my_ring + slot * S::kStageBytes;
+        {
           float s[BK][NT][4];
           // minima: one MMA whose k slots are the groups, sums of q as hi (k < 8) and lo
 #pragma unroll
@@ -622,15 +627,6 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
               }
             }
           }
-          // values' scales and minima (rows = groups), in the order of the weights' operand
-          uint2 vs[BK][NG], mn[BK];
-#pragma unroll
-          for (int kb = 0; kb < BK; ++kb) {
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) vs[kb][gr] = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 576 * NG + gr * 32 + t * 8);
-            mn[kb] = make_uint2(0, 0);
-            if (g < NG) mn[kb] = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 608 * NG + g * 32 + t * 8);
-          }
           // scores in units of log2, less the maximum as far as it is known, plus 7: weights are 2^7 p.  The maximum is raised only when it lags by more than 2^8, so most
           // blocks need no exchange between lanes.
           bool raise = false;
@@ -648,51 +644,43 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
               }
               raise |= top > kPScale + 8.f;
             }
-          bool odd_values = false;           // a scale or minimum of a value that is no number
+          bool odd_values = false;           // a scale or minimum of a value is no number
           if (cut || careful || !ready || __any_sync(0xffffffffu, raise)) {
             if (cut) {
 #pragma unroll
               for (int kb = 0; kb < BK; ++kb) {
-                const bool there = bits >> (k0 + kb) & 1;
+                const bool there = bits >> kb & 1;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                   for (int k = 0; k < 4; ++k) {
-                    const int key = key0 + (k0 + kb) * 16 + g + (k >= 2 ? 8 : 0), c = nt * 8 + 2 * t + (k & 1);
+                    const int key = key0 + kb * 16 + g + (k >= 2 ? 8 : 0), c = nt * 8 + 2 * t + (k & 1);
                     if (key >= col_end[c] || key < col_from[c] || !there) s[kb][nt][k] = -CUDART_INF_F;
                   }
-                if (!there) mn[kb] = make_uint2(0, 0);
-                uint32_t odd = odd_halves(mn[kb].x) | odd_halves(mn[kb].y);
-#pragma unroll
-                for (int gr = 0; gr < NG; ++gr) {
-                  if (!there) vs[kb][gr] = make_uint2(0, 0);
-                  odd |= odd_halves(vs[kb][gr].x) | odd_halves(vs[kb][gr].y);
-                }
-                odd_values |= odd != 0;
-              }
-              odd_values = __any_sync(0xffffffffu, odd_values);
-              if (odd_values) {              // they take no part here; below, the rows that see them get them
-#pragma unroll
-                for (int kb = 0; kb < BK; ++kb) {
-                  mn[kb].x &= ~odd_halves(mn[kb].x);
-                  mn[kb].y &= ~odd_halves(mn[kb].y);
-#pragma unroll
-                  for (int gr = 0; gr < NG; ++gr) {
-                    vs[kb][gr].x &= ~odd_halves(vs[kb][gr].x);
-                    vs[kb][gr].y &= ~odd_halves(vs[kb][gr].y);
+                // What is no number among the values' scales and minima counts for the rows that see its key alone, and nothing counts of a block that is not there.  The stage is this
+                // warp's own, so it is put in order in place, a word per lane: such scales become -0 and their minima 0; below, the rows that give a -0 a weight get their NaN.
+                uint32_t* scales = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage) + kb * 640 * NG + 576 * NG);
+                for (int i = lane; i < 8 * NG; i += 32) {
+                  const uint32_t sc = scales[i], mi = scales[8 * NG + i], odd = there ? odd_halves(sc) | odd_halves(mi) : 0xffffffffu;
+                  if (odd) {
+                    scales[i] = there ? (sc & ~odd) | (odd & 0x80008000u) : 0u;
+                    scales[8 * NG + i] = mi & ~odd;
+                    odd_values |= there;
                   }
                 }
               }
+              odd_values = __any_sync(0xffffffffu, odd_values);
+              tc::fence_async_smem();        // before the next copy into this stage
             }
             if (careful) {
               __half2 most = __float2half2_rn(0.f);
+              uint32_t* scales = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage) + 576 * NG);
 #pragma unroll
               for (int kb = 0; kb < BK; ++kb)
-#pragma unroll
-                for (int gr = 0; gr < NG; ++gr) most = __hmax2(most, __hmax2(as_half2(vs[kb][gr].x), as_half2(vs[kb][gr].y)));
+                for (int i = lane; i < 8 * NG; i += 32) most = __hmax2(most, as_half2(scales[kb * 160 * NG + i]));
               float x = fmaxf(__low2float(most), __high2float(most));
 #pragma unroll
-              for (int off = 1; off < 4; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+              for (int off = 16; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
               if (x > __uint_as_float((uint32_t)(127 + r) << 23) && x <= 65504.f) {        // above 2^r: weights up to 2^15 times scales up to 1 stay halves
                 const int rn = (int)(__float_as_uint(x) >> 23) - 126;                      // x < 2^rn
                 const float fade = __uint_as_float((uint32_t)(127 + r - rn) << 23);
@@ -704,23 +692,18 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
 #pragma unroll
                     for (int k = 0; k < 4; ++k) o[i][nt][k] *= fade;
               }
-              if (r) {
-                const __half2 down = __float2half2_rn(__uint_as_float((uint32_t)(127 - r) << 23));
+              const __half2 down = __float2half2_rn(__uint_as_float((uint32_t)(127 - r) << 23));
 #pragma unroll
-                for (int kb = 0; kb < BK; ++kb)
-#pragma unroll
-                  for (int gr = 0; gr < NG; ++gr) {
-                    vs[kb][gr].x = as_u32(__hmul2(as_half2(vs[kb][gr].x), down));
-                    vs[kb][gr].y = as_u32(__hmul2(as_half2(vs[kb][gr].y), down));
-                  }
-              }
+              for (int kb = 0; kb < BK; ++kb)
+                for (int i = lane; i < 8 * NG; i += 32) scales[kb * 160 * NG + i] = as_u32(__hmul2(as_half2(scales[kb * 160 * NG + i]), down));
+              tc::fence_async_smem();
             }
+            __syncwarp();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                float x = fmaxf(s[0][nt][k], s[0][nt][k + 2]);
-                if (BK == 2) x = fmaxf(x, fmaxf(s[BK - 1][nt][k], s[BK - 1][nt][k + 2]));
+                float x = fmaxf(fmaxf(s[0][nt][k], s[0][nt][k + 2]), fmaxf(s[1][nt][k], s[1][nt][k + 2]));
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
                 const float rise = x - kPScale;
@@ -742,10 +725,12 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
               }
             ready = __all_sync(0xffffffffu, seen == (1u << (2 * NT)) - 1u);
           }
-          // weights as halves (float32: two of them), from accumulators to B operands; then values
+          // weights as halves (float32: two of them), from accumulators to B operands; then values, whose minima are an operand with groups as rows
 #pragma unroll
           for (int kb = 0; kb < BK; ++kb) {
             uint32_t pb[NT][kSplit ? 4 : 2];
+            uint2 mn = make_uint2(0, 0);
+            if (g < NG) mn = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 608 * NG + g * 32 + t * 8);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               float e[4];
@@ -761,15 +746,14 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                 pb[nt][kSplit ? 2 : 0] = transposed(pack(e[0] - f0.x, e[1] - f0.y));
                 pb[nt][kSplit ? 3 : 0] = transposed(pack(e[2] - f1.x, e[3] - f1.y));
               }
-              if (kSplit) mma_split<false>(om[nt], mn[kb].x, 0u, mn[kb].y, 0u, pb[nt][0], pb[nt][1], pb[nt][kSplit ? 2 : 0], pb[nt][kSplit ? 3 : 0]);
-              else mma_half(om[nt], mn[kb].x, 0u, mn[kb].y, 0u, pb[nt][0], pb[nt][1]);
+              if (kSplit) mma_split<false>(om[nt], mn.x, 0u, mn.y, 0u, pb[nt][0], pb[nt][1], pb[nt][kSplit ? 2 : 0], pb[nt][kSplit ? 3 : 0]);
+              else mma_half(om[nt], mn.x, 0u, mn.y, 0u, pb[nt][0], pb[nt][1]);
             }
-            if (odd_values && (bits >> (k0 + kb) & 1)) {
+            if (odd_values) {
 #pragma unroll
               for (int gr = 0; gr < NG; ++gr) {
-                const uint8_t* block = stage + kb * 640 * NG;
-                const uint2 sc = *reinterpret_cast<const uint2*>(block + 576 * NG + gr * 32 + t * 8), mi = *reinterpret_cast<const uint2*>(block + 608 * NG + gr * 32 + t * 8);
-                const uint32_t ox = odd_halves(sc.x) | odd_halves(mi.x), oy = odd_halves(sc.y) | odd_halves(mi.y);
+                const uint2 sc = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 576 * NG + gr * 32 + t * 8);
+                const uint32_t ox = __vcmpeq2(sc.x, 0x80008000u), oy = __vcmpeq2(sc.y, 0x80008000u);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {            // lane (g, t): row g's weights of keys 2t, 2t + 1, 2t + 8, 2t + 9
                   const unsigned hit = __ballot_sync(0xffffffffu, (pb[nt][0] & ox) | (pb[nt][1] & oy));
@@ -782,11 +766,12 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
               const uint2 w = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 256 * NG + gr * 256 + lane * 8);
+              const uint2 vs = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 576 * NG + gr * 32 + t * 8);        // in the order of the weights' operand
               uint32_t wb[NT][kSplit ? 4 : 2];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 if (kSplit) {
-                  const float2 sx = __half22float2(as_half2(vs[kb][gr].x)), sy = __half22float2(as_half2(vs[kb][gr].y));
+                  const float2 sx = __half22float2(as_half2(vs.x)), sy = __half22float2(as_half2(vs.y));
 #pragma unroll
                   for (int i = 0; i < 2; ++i) {
                     const float2 hi = __half22float2(as_half2(pb[nt][i])), lo = __half22float2(as_half2(pb[nt][kSplit ? 2 + i : 0]));
@@ -796,8 +781,8 @@ __global__ void __launch_bounds__(kThreads, NT >= 3 || NG >= 5 ? 2 : 3) attentio
                     wb[nt][kSplit ? 2 + i : 0] = pack(x - f.x, y - f.y);
                   }
                 } else {
-                  wb[nt][0] = as_u32(__hmul2(as_half2(pb[nt][0]), as_half2(vs[kb][gr].x)));
-                  wb[nt][1] = as_u32(__hmul2(as_half2(pb[nt][1]), as_half2(vs[kb][gr].y)));
+                  wb[nt][0] = as_u32(__hmul2(as_half2(pb[nt][0]), as_half2(vs.x)));
+                  wb[nt][1] = as_u32(__hmul2(as_half2(pb[nt][1]), as_half2(vs.y)));
                 }
               }
 #pragma unroll

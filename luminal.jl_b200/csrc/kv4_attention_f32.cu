@@ -1,18 +1,20 @@
-// Attention over the 4-bit paged cache, f32 queries: the instantiations.
+// Attention over the 4-bit paged cache, float32 queries: the instantiations.
 #include "kv4_attention.cuh"
 
 namespace lmb {
 namespace kv4 {
 namespace {
-Variant g_variants[9][5];
+Variant g_variants[9][kMostTiles + 1];
 }
 const Variant* variant_f32(int NG, int NT) { return &g_variants[NG][NT]; }
 
 int32_t configure_f32() {
-#define KV4_ONE(NG, NT) LMB_TRY((configure_one<float, NG, NT>(&g_variants[NG][NT])))
-#define KV4_BOTH(NG) KV4_ONE(NG, 1); KV4_ONE(NG, 2)
+#define KV4_BOTH(NG)                                            \
+  LMB_TRY((configure_one<float, NG, 1>(&g_variants[NG][1]))); \
+  LMB_TRY((configure_one<float, NG, 2>(&g_variants[NG][2])))
   KV4_BOTH(1); KV4_BOTH(2); KV4_BOTH(3); KV4_BOTH(4);
   KV4_BOTH(5); KV4_BOTH(6); KV4_BOTH(7); KV4_BOTH(8);
+#undef KV4_BOTH
   return LMB200_OK;
 }
 
