@@ -603,8 +603,9 @@ int32_t lmb200_decode_attention_noalloc(lmb200_ctx ctx, int32_t dtype, const voi
  *   then float16, D / 2 each key s, key m [g][t16 % 8][t16 / 8], value s, value m [g][t16 % 8 / 2][t16 / 8][t16 % 2]
  * A slot is page * page_size + place in the page.  The places of a cache that no call has written are the caller's (zeros read back as 0).
  *
- * A slot or a table entry outside the cache, or row offsets outside the rows, touch no memory: they are left out and the next synchronising call
- * returns LMB200_EINVAL.
+ * A slot or a table entry outside the cache, lengths beyond the tables and row offsets that do not ascend within the rows touch no memory: such entries and
+ * sequences are left out (kv4_attention: of offsets that descend or leave the rows, all sequences are), and the next synchronising call returns LMB200_EINVAL.
+ * max_pages * page_size is at most 2^30.
  * ------------------------------------------------------------------------------------------ */
 int32_t lmb200_kv4_page_bytes(int32_t page_size, int32_t n_kv_heads, int32_t head_dim, int64_t* bytes);
 /* Room for add[b] >= 0 more tokens of every sequence b < n_seq (at most 8192).  A sequence of `lens` tokens holds the first ceil(lens / page_size) pages of its row of
@@ -646,7 +647,7 @@ int32_t lmb200_kv4_attention(lmb200_ctx ctx, int32_t dtype, const void* q, int64
  * -infinities takes nothing and gives -1.
  * tokens_out[rows]: per sequence the taken drafts, the new token, then -1 up to its last row; n_out[b]: how many tokens those are (0 for a sequence without rows); drop[b]: how many drafts
  * were refused, for lmb200_kv_shrink.  Rows behind cu_rows[n_seq] are left as they are.  target and draft in dtype (F32 or BF16), rows apart by the strides.  workspace:
- * lmb200_verify_drafts_workspace(rows) bytes, in any state.  Stands beside lmb200_argmax; replaces the choice of one token (src/Decoding.jl:119-124). */
+ * lmb200_verify_drafts_workspace(rows) bytes, in any state.  tokens_out may not be tokens.  Stands beside lmb200_argmax; replaces the choice of one token (src/Decoding.jl:119-124). */
 int32_t lmb200_verify_drafts_workspace(int32_t rows, int64_t* bytes);
 int32_t lmb200_verify_drafts(lmb200_ctx ctx, int32_t dtype, const void* target, int64_t target_stride, const void* draft, int64_t draft_stride, int32_t vocab, int32_t rows,
                              int32_t n_seq, const int32_t* cu_rows, const int32_t* tokens, const float* temperature, const float* accept_u, const float* sample_u,

@@ -47,7 +47,9 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   LMB_TRY(kv4::check_cache("kv4_attention", n_kv_heads, head_dim, n_pages, page_size));
   LMB_REQUIRE(group >= 1 && (int64_t)n_kv_heads * group <= 65535, "kv4_attention: %d query heads for each of %d kv heads", group, n_kv_heads);
   LMB_REQUIRE(rows >= 0 && n_seq >= 1 && n_seq <= 8192 && window >= 0, "kv4_attention: %d rows, %d sequences (1 to 8192), window %d", rows, n_seq, window);
-  LMB_REQUIRE(max_pages >= 1 && (int64_t)max_pages * page_size <= INT32_MAX, "kv4_attention: block tables of %d pages", max_pages);
+  const int64_t capacity = (int64_t)max_pages * page_size;
+  LMB_REQUIRE(max_pages >= 1 && capacity <= kv4::kMostTokens, "kv4_attention: block tables of %d pages (up to 2^30 tokens)", max_pages);
+  LMB_REQUIRE(rows <= kv4::kMostTokens && (int64_t)rows * group <= INT32_MAX, "kv4_attention: %d rows for each of %d heads", rows, group);
   LMB_REQUIRE(rows == 0 || (q && out && cu_rows && lens && table && pages && workspace), "kv4_attention: null pointer");
   const int64_t width = (int64_t)n_kv_heads * group * head_dim;
   LMB_REQUIRE(q_stride >= width && out_stride >= width, "kv4_attention: row strides %lld and %lld for rows of %lld elements", (long long)q_stride, (long long)out_stride,
@@ -67,14 +69,14 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   const int NT = ceil_div(each, 16) * 5 <= ceil_div(each, 8) * 3 ? 2 : 1;
   const kv4::Variant* v = f32 ? kv4::variant_f32(NG, NT) : kv4::variant_bf16(NG, NT);
   // units of work are counted in 32 bits
-  const int64_t tiles = ceil_div((int64_t)rows * group, 8 * NT) + std::min(n_seq, rows), units = ceil_div((int64_t)max_pages * page_size, kv4::kUnit) + 1;
+  const int64_t tiles = ceil_div((int64_t)rows * group, 8 * NT) + std::min(n_seq, rows), units = ceil_div(capacity, kv4::kUnit) + 1;
   LMB_REQUIRE(tiles * n_kv_heads <= UINT32_MAX / units, "kv4_attention: %d rows of %d heads over %d pages are too many for one call", rows, n_kv_heads * group, max_pages);
   LMB_CUDA(cudaSetDevice(ctx->device));
   const int grid = (int)std::min<int64_t>(grid_of(ctx, v), tiles * n_kv_heads * units);
   kv4::Params p = {};
   p.q = q; p.out = out; p.q_stride = q_stride; p.out_stride = out_stride;
   p.rows = rows; p.n_seq = n_seq; p.max_pages = max_pages; p.n_pages = n_pages; p.shift = kv4::page_shift(page_size);
-  p.heads = n_kv_heads; p.G = group; p.window = window;
+  p.heads = n_kv_heads; p.G = group; p.window = window < capacity ? window : 0;
   p.scale = scale * 1.4426950408889634f;
   p.cu_rows = cu_rows; p.lens = lens; p.table = table;
   p.pages = static_cast<const uint8_t*>(pages);

@@ -23,7 +23,7 @@ namespace lmb {
 namespace kv4 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kUnit = 128, kMaxSeqs = 8192;
-constexpr int kCounters = 4096, kMostShares = kCounters / 2, kJoin = 16;
+constexpr int kCounters = 2048, kMostShares = kCounters / 2, kJoin = 16;
 constexpr unsigned kLonger = 8;                    // units by which a piece may be longer than a share
 
 struct Params {
@@ -35,7 +35,7 @@ struct Params {
   const int *cu_rows, *lens, *table;
   const uint8_t* pages;
   int* dev_err;
-  unsigned* counters;                        // [kCounters], zero between calls: two per share
+  unsigned* counters;                        // [kCounters], zero between calls: per share one for all of a triple's shares and one for a group of them
   float2* part_ml;                           // [share][2][columns]: maximum (log2) and sum
   float* part_o;                             // [share][2][columns][D]
 };
@@ -62,6 +62,7 @@ template <typename T, int NG, int NT> struct Shape {
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kPitch = D + 4;                    // of the joined sums: 2 kPitch = 8 banks
   static constexpr int kMerge = 2 * COLS * kPitch * 4;
+  static_assert(kMerge >= kMostShares / kJoin * COLS * 4, "join_parts keeps a weight per part and row there");
   static constexpr int kQ = 2 * NG * NT * 32 * (kSplit ? 16 : 8);
   static constexpr int kQSum = NT * 32 * 8;
   static constexpr int kFixed = kRing + kMerge + kQ + kQSum + COLS * 16 + 2 * kWarps * COLS * 4 + kWarps * kStages * 8 + 64 + 3 * 96 + kWarps * 16;
@@ -179,20 +180,20 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
     const int per = (p.n_seq + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, p.n_seq), b1 = min(b0 + per, p.n_seq);
     unsigned sum = 0, items = 0;
-    bool bad = false;
+    bool bad = false, broken = false;
     for (int b = b0; b < b1; ++b) {
       const int r0 = p.cu_rows[b], r1 = p.cu_rows[b + 1], l = p.lens[b];
       const int len = min(max(l, 0), capacity);
       int T_ = r1 - r0, first;
       bad |= l != len;
-      if (r0 < 0 || r1 < r0 || r1 > p.rows) { bad = true; T_ = 0; }
+      if (r0 < 0 || r1 < r0 || r1 > p.rows) { broken = true; T_ = 0; }
       const unsigned triples = T_ > 0 ? (unsigned)row_tiles(T_, p.G, COLS) * p.heads : 0u, n = triples * units_of(T_, len, first);
       seq_len[b] = len;
       before[b + 1] = n;
       sum += n;
       items += triples;
     }
-    if (bad && blockIdx.x == 0) atomicExch(p.dev_err, kErrPage);
+    if ((bad || broken) && blockIdx.x == 0) atomicExch(p.dev_err, kErrPage);
     // units per piece: 1, or so many that every CTA has one piece
     {
       unsigned all = sum, of = items;
@@ -202,7 +203,8 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
         of += __shfl_xor_sync(0xffffffffu, of, off);
       }
       if (lane == 0) { shared_word[warp] = (int)all; shared_word[8 + warp] = (int)of; }
-      __syncthreads();
+      // Offsets that descend could make sequences overlap, and more work than the host has counted.
+      if (__syncthreads_or(broken)) return;
       all = of = 0;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) { all += (unsigned)shared_word[w]; of += (unsigned)shared_word[8 + w]; }
@@ -261,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
     const int rows0 = p.cu_rows[b], T_ = p.cu_rows[b + 1] - rows0, len = seq_len[b];
     const int n_units = units_of(T_, len, first_unit);
     const int n_pieces = (n_units + (int)piece - 1) / (int)piece;        // of as equal lengths as units allow
-    const int triple = (int)(u - before[b]) / n_pieces, tile = triple / p.heads, head = triple - tile * p.heads;
+    const int triple = (int)((unsigned)(u - before[b]) / (unsigned)n_pieces), tile = triple / p.heads, head = triple - tile * p.heads;
     const int64_t item0 = (int64_t)before[b] + (int64_t)triple * n_pieces;
     const int valid = min(COLS, T_ * p.G - tile * COLS);                 // query rows of this tile; their positions ascend
     const int first_pos = len - T_ + tile * COLS / p.G, last_pos = len - T_ + (tile * COLS + valid - 1) / p.G;
@@ -537,30 +539,29 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
     uint32_t seen;                           // columns that have a maximum; m of the others is 0
     const int n_stages = sg->n_stages, first_key = (sg->first_block + 2 * warp) * 16, all_from = sg->all_from, all_to = sg->all_to;
     for (bool careful = false;; careful = true) {
-    r = 0;
-    seen = 0;
-    bool ready = false;                      // all columns have one
+      r = 0;
+      seen = 0;
+      bool ready = false;                    // all columns have one
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = 0.f;
-      l[nt][0] = l[nt][1] = 0.f;
+      for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = 0.f;
+        l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) om[nt][k] = 0.f;
+        for (int k = 0; k < 4; ++k) om[nt][k] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2 * NG; ++i)
+        for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
-    }
+          for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
+      }
 #pragma unroll 1
-    for (int j = 0; j < n_stages; ++j) {
-      const uint32_t bits = loaded >> (2 * slot) & 3u;
-      if (bits) {
-        tc::mbar_wait(my_full + slot, phases >> slot & 1u, dead, p.dev_err);
-        phases ^= 1u << slot;
-        const int key0 = first_key + j * kUnit;
-        const bool cut = bits != 3u || key0 < all_from || key0 + 32 > all_to;              // some row does not see all of it
-        const uint8_t* stage = my_ring + slot * S::kStageBytes;
-        {
+      for (int j = 0; j < n_stages; ++j) {
+        const uint32_t bits = loaded >> (2 * slot) & 3u;
+        if (bits) {
+          tc::mbar_wait(my_full + slot, phases >> slot & 1u, dead, p.dev_err);
+          phases ^= 1u << slot;
+          const int key0 = first_key + j * kUnit;
+          const bool cut = bits != 3u || key0 < all_from || key0 + 32 > all_to;              // some row does not see all of it
+          const uint8_t* stage = my_ring + slot * S::kStageBytes;
           float s[BK][NT][4];
           // minima: one MMA whose k slots are the groups, sums of q as hi (k < 8) and lo
 #pragma unroll
@@ -677,11 +678,14 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
               uint32_t* scales = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage) + 576 * NG);
 #pragma unroll
               for (int kb = 0; kb < BK; ++kb)
-                for (int i = lane; i < 8 * NG; i += 32) most = __hmax2(most, as_half2(scales[kb * 160 * NG + i]));
+                for (int i = lane; i < 8 * NG; i += 32) {
+                  const uint32_t sc = scales[kb * 160 * NG + i];
+                  most = __hmax2(most, as_half2(sc & ~odd_halves(sc)));
+                }
               float x = fmaxf(__low2float(most), __high2float(most));
 #pragma unroll
               for (int off = 16; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-              if (x > __uint_as_float((uint32_t)(127 + r) << 23) && x <= 65504.f) {        // above 2^r: weights up to 2^15 times scales up to 1 stay halves
+              if (x > __uint_as_float((uint32_t)(127 + r) << 23)) {        // above 2^r: weights up to 2^15 times scales up to 1 stay halves
                 const int rn = (int)(__float_as_uint(x) >> 23) - 126;                      // x < 2^rn
                 const float fade = __uint_as_float((uint32_t)(127 + r - rn) << 23);
                 r = rn;
@@ -799,22 +803,21 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
             }
           }
         }
+        __syncwarp();
+        if (j + kStages < n_stages) issue(sg, j + kStages, slot);
+        slot = slot + 1 == kStages ? 0 : slot + 1;
       }
-      __syncwarp();
-      if (j + kStages < n_stages) issue(sg, j + kStages, slot);
-      slot = slot + 1 == kStages ? 0 : slot + 1;
-    }
 
-    float all = 0.f;
+      float all = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 4; ++k) {
 #pragma unroll
-        for (int i = 0; i < 2 * NG; ++i) all = fmaf(o[i][nt][k], 0.f, all);
-      }
-    if (careful || !__any_sync(0xffffffffu, all != 0.f)) break;          // NaN is not 0 either
-    start(sg, page_at(sg, 0), page_at(sg, 1));
+          for (int i = 0; i < 2 * NG; ++i) all = fmaf(o[i][nt][k], 0.f, all);
+        }
+      if (careful || !__any_sync(0xffffffffu, all != 0.f)) break;          // NaN is not 0 either
+      start(sg, page_at(sg, 0), page_at(sg, 1));
     }
 
     // ---- the next segment's keys are asked for while this one's sums become one -------------------------------------------------

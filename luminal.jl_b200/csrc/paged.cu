@@ -620,7 +620,7 @@ cudaError_t launch_cluster(K kernel, int ctas, size_t smem, cudaStream_t st, con
 
 int32_t check_tables(const char* who, int n_seq, int page, int max_pages, int n_pages) {
   LMB_REQUIRE(n_seq >= 1 && n_seq <= kMaxSeqs, "%s: %d sequences (1 to %d)", who, n_seq, kMaxSeqs);
-  LMB_REQUIRE(max_pages >= 1, "%s: block tables of %d pages", who, max_pages);
+  LMB_REQUIRE(max_pages >= 1 && (int64_t)max_pages * page <= kv4::kMostTokens, "%s: block tables of %d pages (up to 2^30 tokens)", who, max_pages);
   return kv4::check_cache(who, 1, 32, n_pages, page);
 }
 
@@ -698,7 +698,7 @@ extern "C" int32_t lmb200_kv_reserve(lmb200_ctx h, int32_t n_seq, int32_t page_s
   Ctx* ctx = ctx_from(h);
   if (!ctx) return LMB200_EINVAL;
   LMB_TRY(check_tables("kv_reserve", n_seq, page_size, max_pages, n_pages));
-  LMB_REQUIRE(rows >= 0, "kv_reserve: %d rows", rows);
+  LMB_REQUIRE(rows >= 0 && rows <= kv4::kMostTokens, "kv_reserve: %d rows (up to 2^30)", rows);
   LMB_REQUIRE(lens && add && table && free_list && n_free && lens_out && n_free_out && cu_rows && status && (slots || rows == 0), "kv_reserve: null pointer");
   LMB_CUDA(cudaSetDevice(ctx->device));
   TableParams p = {n_seq, kv4::page_shift(page_size), max_pages, n_pages, rows, lens, add, n_free, table, const_cast<int32_t*>(free_list),

@@ -732,6 +732,7 @@ extern "C" int32_t lmb200_verify_drafts(lmb200_ctx h, int32_t dtype, const void*
   int64_t need = 0;
   LMB_TRY(lmb200_verify_drafts_workspace(rows, &need));
   LMB_REQUIRE(rows == 0 || workspace_bytes >= need, "verify_drafts: a workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+  LMB_REQUIRE(rows == 0 || tokens_out != tokens, "verify_drafts: tokens_out may not be tokens");
   LMB_CUDA(cudaSetDevice(ctx->device));
   if (rows == 0) {
     LMB_CUDA(cudaMemsetAsync(n_out, 0, (size_t)n_seq * 4, ctx->stream));

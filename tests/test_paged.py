@@ -72,7 +72,8 @@ def _args(**change):
 @pytest.mark.parametrize("change", [dict(dtype=2), dict(q=0), dict(out=0), dict(cu=0), dict(lens=0), dict(table=0), dict(pages=0), dict(ws=0), dict(q_stride=511), dict(out_stride=500),
                                     dict(q_stride=516), dict(q=258), dict(out=264 + 4), dict(rows=-1), dict(n_seq=0), dict(n_seq=8193), dict(max_pages=0),
                                     dict(max_pages=1 << 28), dict(n_pages=0), dict(n_pages=1 << 28), dict(page=24), dict(heads=0), dict(group=0), dict(group=1 << 20), dict(D=64 + 16),
-                                    dict(D=512), dict(window=-1), dict(ws_bytes=0), dict(ws=260)])
+                                    dict(D=512), dict(window=-1), dict(ws_bytes=0), dict(ws=260), dict(max_pages=(1 << 26) + 1), dict(rows=(1 << 30) + 1),
+                                    dict(rows=1 << 29, group=4, q_stride=1024, out_stride=1024)])
 def test_attention_refuses(lib_built, change):
     from importlib import import_module
     _lib = import_module("luminal_jl_b200._lib")
@@ -98,7 +99,8 @@ def test_store_refuses(lib_built, name, change):
 
 
 @pytest.mark.parametrize("change", [dict(n_seq=0), dict(n_seq=8193), dict(page=20), dict(max_pages=0), dict(n_pages=0), dict(n_pages=1 << 28), dict(rows=-1), dict(lens=0), dict(add=0),
-                                    dict(table=0), dict(free=0), dict(n_free=0), dict(lens_out=0), dict(n_free_out=0), dict(cu=0), dict(slots=0), dict(status=0)])
+                                    dict(table=0), dict(free=0), dict(n_free=0), dict(lens_out=0), dict(n_free_out=0), dict(cu=0), dict(slots=0), dict(status=0), dict(max_pages=(1 << 26) + 1),
+                                    dict(rows=(1 << 30) + 1)])
 def test_reserve_and_shrink_refuse(lib_built, change):
     from importlib import import_module
     _lib = import_module("luminal_jl_b200._lib")
@@ -115,11 +117,11 @@ def test_reserve_and_shrink_refuse(lib_built, change):
 
 
 @pytest.mark.parametrize("change", [dict(dtype=2), dict(target=0), dict(target=258), dict(draft=257), dict(ts=99), dict(ds=99), dict(vocab=0), dict(rows=-1), dict(rows=70000), dict(n_seq=0),
-                                    dict(cu=0), dict(tokens=0), dict(au=0), dict(su=0), dict(out=0), dict(n_out=0), dict(drop=0), dict(ws=0), dict(ws=264), dict(ws_bytes=100)])
+                                    dict(cu=0), dict(tokens=0), dict(au=0), dict(su=0), dict(out=0), dict(n_out=0), dict(drop=0), dict(ws=0), dict(ws=264), dict(ws_bytes=100), dict(out=256)])
 def test_verify_refuses(lib_built, change):
     from importlib import import_module
     _lib = import_module("luminal_jl_b200._lib")
-    a = dict(dtype=0, target=256, ts=100, draft=256, ds=100, vocab=100, rows=5, n_seq=2, cu=256, tokens=256, T=256, au=256, su=256, out=256, n_out=256, drop=256, ws=256, ws_bytes=1 << 30)
+    a = dict(dtype=0, target=256, ts=100, draft=256, ds=100, vocab=100, rows=5, n_seq=2, cu=256, tokens=256, T=256, au=256, su=256, out=512, n_out=256, drop=256, ws=256, ws_bytes=1 << 30)
     a.update(change)
     with pytest.raises(lib_built.LuminalB200Error) as e:
         _lib.call("lmb200_verify_drafts", FakeContext().handle, *a.values())
@@ -560,6 +562,57 @@ def test_attention_row_offsets_and_lengths_that_do_not_fit(on_torch, cu, lens):
     with pytest.raises(L.LuminalB200Error) as e:
         dev.sync()
     assert e.value.code == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu", [[0, 3, 1, 3], [0, 1, 2, 4], [0, 3, 0, 3]])
+def test_attention_offsets_that_descend_or_leave_the_rows_write_nothing(on_torch, cu):
+    """Overlapping sequences would be more work than the rows can hold, so the whole call is left out; the workspace stays usable."""
+    import torch
+    L, dev = on_torch
+    q, good, lens, table, pages = one_case(np.random.default_rng(5), "bf16", lens=(70, 300, 40), new=(1, 1, 1))
+    out, ws = attend(L, dev, q, cuda(np.array(cu, np.int32)), cuda(lens), cuda(table), cuda(pages), 16, 0.1)
+    with pytest.raises(L.LuminalB200Error) as e:
+        dev.sync()
+    assert e.value.code == -1 and (out == 7).all()
+    a, _ = attend(L, dev, q, cuda(good), cuda(lens), cuda(table), cuda(pages), 16, 0.1, ws=ws)
+    b, _ = attend(L, dev, q, cuda(good), cuda(lens), cuda(table), cuda(pages), 16, 0.1)
+    dev.sync()
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 320, 304, 303])
+def test_attention_windows_that_reach_past_everything(on_torch, window):
+    """A window as long as the table or longer is none, also for rows before a sequence's first token."""
+    import torch
+    L, dev = on_torch
+    q, cu, _, table, pages = one_case(np.random.default_rng(7), "bf16", new=(2, 5))
+    assert table.shape[1] * 16 == 304
+    lens = np.array([1, 2], np.int32)
+    none, _ = attend(L, dev, q, cuda(cu), cuda(lens), cuda(table), cuda(pages), 16, 0.1)
+    out, _ = attend(L, dev, q, cuda(cu), cuda(lens), cuda(table), cuda(pages), 16, 0.1, window=window)
+    dev.sync()
+    assert torch.equal(out, none) and (out[[0, 2, 3, 4]] == 0).all() and (out[[1, 5, 6]] != 0).any(-1).any(-1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_an_infinite_scale_spoils_its_features_alone(on_torch, dtype):
+    """Beside scales that want the second pass: those are scaled down by the largest number among them."""
+    L, dev = on_torch
+    q, cu, lens, table, pages = one_case(np.random.default_rng(8), dtype, lens=(70, 600), new=(3, 1))
+    meta = pages[..., 16 * 128:].view(np.float16).reshape(*pages.shape[:3], 2, 2, 64)
+    meta[..., 1, :, :] = np.clip(meta[..., 1, :, :].astype(np.float32) * 9000, -60000, 60000)
+    want, size = P.attention(q.float().cpu().numpy(), cu, lens, table, pages, 16, 128 ** -0.5)
+    _, _, _, _, vm = P.places(128)
+    pages[table[1, 2], :, 0, 16 * 128:].view(np.float16)[:, vm[7, 2]] = np.inf
+    out, _ = attend(L, dev, q, cuda(cu), cuda(lens), cuda(table), cuda(pages), 16, 128 ** -0.5)
+    dev.sync()
+    assert not out[3, :, 64:96].isfinite().any()
+    out[3, :, 64:96] = 0
+    want[3, :, 64:96] = 0
+    check(out, want, size, dtype)
 
 
 @pytest.mark.gpu
