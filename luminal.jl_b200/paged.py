@@ -36,6 +36,22 @@ def _code(a):
         return _CODES.setdefault(a.dtype, _NAMES.get(str(a.dtype), -1))
 
 
+def _here(device, *arrays):
+    """Refuses arrays of another GPU than the device's: a kernel would fault on them."""
+    for a in arrays:
+        if a is None:
+            continue
+        if isinstance(a, DeviceArray):
+            on = a.device.ordinal
+        else:
+            on = getattr(a, "get_device", None)
+            if on is None:
+                continue
+            on = on()
+        if on >= 0 and on != device.ordinal:               # below 0: host memory, refused by name below
+            raise ValueError(f"an array on GPU {on} for a device on GPU {device.ordinal}")
+
+
 def _count(a):
     try:
         return a.numel()
@@ -120,6 +136,7 @@ def _pool(pages, page_size, heads, dim):
 
 def kv_reserve(device, lens, add, table, free_list, n_free, *, page_size, lens_out, n_free_out, cu_rows, slots, status):
     """Pages, slots and lengths for add[b] more tokens of every sequence (lmb200_kv_reserve).  lens_out may be lens, n_free_out n_free."""
+    _here(device, lens, add, table, free_list, n_free, lens_out, n_free_out, cu_rows, slots, status)
     n, rows = lens.shape[0], slots.shape[0]
     _call("lmb200_kv_reserve", device.handle, n, page_size, table.shape[1], free_list.shape[0], rows, _ints("lens", lens, n), _ints("add", add, n),
               _ints("table", table, n * table.shape[1]), _ints("free_list", free_list, 1), _ints("n_free", n_free, 1), _ints("lens_out", lens_out, n),
@@ -128,6 +145,7 @@ def kv_reserve(device, lens, add, table, free_list, n_free, *, page_size, lens_o
 
 def kv_shrink(device, lens, drop, table, free_list, n_free, *, page_size, lens_out, n_free_out):
     """The last drop[b] tokens of every sequence leave the cache and their pages go back (lmb200_kv_shrink)."""
+    _here(device, lens, drop, table, free_list, n_free, lens_out, n_free_out)
     n = lens.shape[0]
     _call("lmb200_kv_shrink", device.handle, n, page_size, table.shape[1], free_list.shape[0], _ints("lens", lens, n), _ints("drop", drop, n),
               _ints("table", table, n * table.shape[1]), _ints("free_list", free_list, 1), _ints("n_free", n_free, 1), _ints("lens_out", lens_out, n),
@@ -135,6 +153,7 @@ def kv_shrink(device, lens, drop, table, free_list, n_free, *, page_size, lens_o
 
 
 def _store(name, device, k, v, slots, pages, page_size):
+    _here(device, k, v, slots, pages)
     rows, heads, dim = k.shape
     (kp, code), (vp, v_code) = _float("k", k), _float("v", v)
     if code != v_code or v.shape != k.shape:
@@ -163,6 +182,7 @@ def kv4_attention_workspace(device, head_dim):
 
 def kv4_attention(device, q, out, cu_rows, lens, table, pages, *, page_size, workspace, scale=None, window=0):
     """Causal attention of the sequences' last tokens, q and out [rows, heads, head_dim], over the cache (lmb200_kv4_attention)."""
+    _here(device, q, out, cu_rows, lens, table, pages, workspace)
     rows, n_heads, dim = q.shape
     n = lens.shape[0]
     (qp, code), (op, out_code) = _float("q", q), _float("out", out)
@@ -174,7 +194,7 @@ def kv4_attention(device, q, out, cu_rows, lens, table, pages, *, page_size, wor
     pool, n_pages = _pool(pages, page_size, heads, dim)
     _call("lmb200_kv4_attention", device.handle, code, qp, _rows("q", q, n_heads * dim), op, _rows("out", out, n_heads * dim), rows, n, _ints("cu_rows", cu_rows, n + 1),
               _ints("lens", lens, n), _ints("table", table, n * table.shape[1]), table.shape[1], pool, n_pages, page_size, heads, n_heads // heads, dim,
-              dim ** -0.5 if scale is None else scale, window, _address("workspace", workspace), _bytes(workspace))
+              dim ** -0.5 if scale is None else scale, window, _plain("workspace", workspace, 0), _bytes(workspace))
 
 
 def verify_drafts_workspace(rows):
@@ -187,6 +207,7 @@ def verify_drafts_workspace(rows):
 def verify_drafts(device, target, draft, cu_rows, tokens, temperature, accept_u, sample_u, tokens_out, n_out, drop, *, workspace):
     """Judges drafted tokens by the target's logits [rows, vocab] (lmb200_verify_drafts).  draft: the draft model's logits, or None for drafts that were certain;
     temperature: one per sequence, or None for the largest logit everywhere."""
+    _here(device, target, draft, cu_rows, tokens, temperature, accept_u, sample_u, tokens_out, n_out, drop, workspace)
     rows, vocab = target.shape
     n = n_out.shape[0]
     tp, code = _float("target", target)
@@ -206,7 +227,7 @@ def verify_drafts(device, target, draft, cu_rows, tokens, temperature, accept_u,
         randoms.append(_plain(what, a, least))
     _call("lmb200_verify_drafts", device.handle, code, tp, _rows("target", target, vocab), dp, d_stride, vocab, rows, n, _ints("cu_rows", cu_rows, n + 1),
               _ints("tokens", tokens, rows), *randoms, _ints("tokens_out", tokens_out, rows), _ints("n_out", n_out, n), _ints("drop", drop, n),
-              _address("workspace", workspace), _bytes(workspace))
+              _plain("workspace", workspace, 0), _bytes(workspace))
 
 
 __all__ = ["kv4_page_bytes", "kv_reserve", "kv_shrink", "kv4_append", "kv4_read", "kv4_attention_workspace", "kv4_attention", "verify_drafts_workspace", "verify_drafts"]

@@ -181,6 +181,41 @@ def test_wrappers_refuse_arrays_that_do_not_fit(lib_built):
             pytest.fail(f"call {i} was not refused")
 
 
+def test_wrappers_refuse_arrays_of_another_gpu(lib_built):
+    import torch
+    L = lib_built
+
+    class Dev:
+        handle, ordinal = FakeContext().handle, 0
+
+    class On:
+        def __init__(self, gpu, *shape, dtype=torch.int32):
+            self.gpu, self.shape, self.dtype, self.is_cuda = gpu, shape, dtype, True
+
+        def get_device(self): return self.gpu
+        def data_ptr(self): return 256
+        def numel(self): return int(np.prod(self.shape))
+        def is_contiguous(self): return True
+        def element_size(self): return 4
+
+    def calls(g):
+        i = iter(g)
+        a = lambda *shape, dtype=torch.int32: On(next(i), *shape, dtype=dtype)  # noqa: E731
+        f = torch.float32
+        yield 4, lambda: L.kv4_append(Dev, a(3, 2, 64, dtype=f), a(3, 2, 64, dtype=f), a(3), a(4, 2, 1, 320), page_size=16)
+        yield 4, lambda: L.kv4_read(Dev, a(3, 2, 64, dtype=f), a(3, 2, 64, dtype=f), a(3), a(4, 2, 1, 320), page_size=16)
+        yield 10, lambda: L.kv_reserve(Dev, a(2), a(2), a(2, 4), a(9), a(1), page_size=16, lens_out=a(2), n_free_out=a(1), cu_rows=a(3), slots=a(5), status=a(1))
+        yield 7, lambda: L.kv_shrink(Dev, a(2), a(2), a(2, 4), a(9), a(1), page_size=16, lens_out=a(2), n_free_out=a(1))
+        yield 7, lambda: L.kv4_attention(Dev, a(3, 4, 64, dtype=f), a(3, 4, 64, dtype=f), a(3), a(2), a(2, 5), a(4, 2, 1, 320), page_size=16, workspace=a(1 << 20))
+        yield 11, lambda: L.verify_drafts(Dev, a(3, 50, dtype=f), a(3, 50, dtype=f), a(2), a(3), a(1, dtype=f), a(3, dtype=f), a(1, dtype=f), a(3), a(1), a(1), workspace=a(1 << 20))
+
+    for which, (n, _) in enumerate(calls([])):
+        for other in range(n):
+            f = list(calls([int(k == other) for k in range(n)]))[which][1]
+            with pytest.raises(ValueError, match="on GPU 1"):
+                f()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # on the GPU
 # ---------------------------------------------------------------------------------------------------------------------
