@@ -468,4 +468,76 @@ comm_init!(d::B200Device, n::Integer, rank::Integer, id::Vector{UInt8}) =
 comm_resync!(d::B200Device) = check(ccall((:lmb200_comm_resync, LIB), Int32, (UInt64,), d.ctx))
 comm_destroy!(d::B200Device) = check(ccall((:lmb200_comm_destroy, LIB), Int32, (UInt64,), d.ctx))
 
+# ---------------------------------------------------------------------------------------------
+# serving many sequences: the paged 4-bit cache, its block tables and drafted tokens.  Arrays are raw device pointers
+# (CUDA.jl: convert(Ptr{Cvoid}, pointer(a))), row-major as the header has them; calls are asynchronous on the context's stream.
+# ---------------------------------------------------------------------------------------------
+struct KVPool                                      # one layer's cache
+    pages::Ptr{Cvoid}
+    n_pages::Int32
+    page_size::Int32
+    n_kv_heads::Int32
+    head_dim::Int32
+end
+function kv4_page_bytes(page_size::Integer, n_kv_heads::Integer, head_dim::Integer)
+    n = Ref{Int64}(0)
+    check(ccall((:lmb200_kv4_page_bytes, LIB), Int32, (Int32, Int32, Int32, Ref{Int64}), page_size, n_kv_heads, head_dim, n))
+    n[]
+end
+struct KVTables                                    # of n_seq sequences: lengths, block tables [n_seq, max_pages], free list [n_pages]
+    n_seq::Int32
+    page_size::Int32
+    max_pages::Int32
+    n_pages::Int32
+    lens::Ptr{Cvoid}
+    table::Ptr{Cvoid}
+    free_list::Ptr{Cvoid}
+    n_free::Ptr{Cvoid}
+end
+"""Room for `add[b]` more tokens of every sequence; lengths and free count are advanced in place (status != 0: nothing is)."""
+kv_reserve!(d::B200Device, t::KVTables, add::Ptr{Cvoid}, rows::Integer, cu_rows::Ptr{Cvoid}, slots::Ptr{Cvoid}, status::Ptr{Cvoid}) =
+    check(ccall((:lmb200_kv_reserve, LIB), Int32,
+                (UInt64, Int32, Int32, Int32, Int32, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+                d.ctx, t.n_seq, t.page_size, t.max_pages, t.n_pages, rows, t.lens, add, t.table, t.free_list, t.n_free, t.lens, t.n_free, cu_rows, slots, status))
+"""The last `drop[b]` tokens of every sequence leave the cache, in place."""
+kv_shrink!(d::B200Device, t::KVTables, drop::Ptr{Cvoid}) =
+    check(ccall((:lmb200_kv_shrink, LIB), Int32,
+                (UInt64, Int32, Int32, Int32, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+                d.ctx, t.n_seq, t.page_size, t.max_pages, t.n_pages, t.lens, drop, t.table, t.free_list, t.n_free, t.lens, t.n_free))
+"""k and v [rows, n_kv_heads, head_dim], rows k_stride / v_stride elements apart, into the cache at slots [rows]."""
+kv4_append!(d::B200Device, c::KVPool, dtype::Integer, k::Ptr{Cvoid}, v::Ptr{Cvoid}, k_stride::Integer, v_stride::Integer, rows::Integer, slots::Ptr{Cvoid}) =
+    check(ccall((:lmb200_kv4_append, LIB), Int32,
+                (UInt64, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int32, Int32, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int32),
+                d.ctx, dtype, k, v, k_stride, v_stride, rows, c.n_kv_heads, c.head_dim, slots, c.pages, c.n_pages, c.page_size))
+"""The values that the cache holds at slots [rows]."""
+kv4_read!(d::B200Device, c::KVPool, dtype::Integer, k_out::Ptr{Cvoid}, v_out::Ptr{Cvoid}, k_stride::Integer, v_stride::Integer, rows::Integer, slots::Ptr{Cvoid}) =
+    check(ccall((:lmb200_kv4_read, LIB), Int32,
+                (UInt64, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int32, Int32, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int32),
+                d.ctx, dtype, k_out, v_out, k_stride, v_stride, rows, c.n_kv_heads, c.head_dim, slots, c.pages, c.n_pages, c.page_size))
+function kv4_attention_workspace(d::B200Device, head_dim::Integer)
+    n = Ref{Int64}(0)
+    check(ccall((:lmb200_kv4_attention_workspace, LIB), Int32, (UInt64, Int32, Ref{Int64}), d.ctx, head_dim, n))
+    n[]
+end
+"""Causal attention of the sequences' last tokens over the cache; the workspace is zero before its first use."""
+kv4_attention!(d::B200Device, c::KVPool, t::KVTables, dtype::Integer, out::Ptr{Cvoid}, out_stride::Integer, q::Ptr{Cvoid}, q_stride::Integer, rows::Integer, group::Integer,
+               cu_rows::Ptr{Cvoid}, workspace::Ptr{Cvoid}, workspace_bytes::Integer; scale::Real=1 / sqrt(c.head_dim), window::Integer=0) =
+    check(ccall((:lmb200_kv4_attention, LIB), Int32,
+                (UInt64, Int32, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Int32, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Ptr{Cvoid}, Int32, Int32, Int32, Int32, Int32, Float32, Int32, Ptr{Cvoid}, Int64),
+                d.ctx, dtype, q, q_stride, out, out_stride, rows, t.n_seq, cu_rows, t.lens, t.table, t.max_pages, c.pages, c.n_pages, c.page_size, c.n_kv_heads, group,
+                c.head_dim, scale, window, workspace, workspace_bytes))
+function verify_drafts_workspace(rows::Integer)
+    n = Ref{Int64}(0)
+    check(ccall((:lmb200_verify_drafts_workspace, LIB), Int32, (Int32, Ref{Int64}), rows, n))
+    n[]
+end
+"""Judges drafted tokens by the target model's logits [rows, vocab] (in place of the argmax of src/Decoding.jl:119-124); draft and temperature may be C_NULL."""
+verify_drafts!(d::B200Device, dtype::Integer, target::Ptr{Cvoid}, target_stride::Integer, draft::Ptr{Cvoid}, draft_stride::Integer, vocab::Integer, rows::Integer, n_seq::Integer,
+               cu_rows::Ptr{Cvoid}, tokens::Ptr{Cvoid}, temperature::Ptr{Cvoid}, accept_u::Ptr{Cvoid}, sample_u::Ptr{Cvoid}, tokens_out::Ptr{Cvoid}, n_out::Ptr{Cvoid}, drop::Ptr{Cvoid}, workspace::Ptr{Cvoid},
+               workspace_bytes::Integer) =
+    check(ccall((:lmb200_verify_drafts, LIB), Int32,
+                (UInt64, Int32, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Int32, Int32, Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64),
+                d.ctx, dtype, target, target_stride, draft, draft_stride, vocab, rows, n_seq, cu_rows, tokens, temperature, accept_u, sample_u, tokens_out, n_out, drop, workspace,
+                workspace_bytes))
+
 end # module B200
