@@ -1,6 +1,8 @@
 // Block tables on the GPU (lmb200_kv_reserve, lmb200_kv_shrink) and the 4-bit cache's store and load (lmb200_kv4_append, lmb200_kv4_read).
 #include <limits.h>
 
+#include <algorithm>
+
 #include "kv4.cuh"
 #include "pdl.cuh"
 
@@ -281,6 +283,19 @@ template <> struct Group<__nv_bfloat16> {
   }
 };
 
+__device__ __forceinline__ uint64_t as_pair(float2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
+__device__ __forceinline__ float2 of_pair(uint64_t u) { return make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32))); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)));
+  return of_pair(d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
+  return of_pair(d);
+}
+
 // n of one value: rint of the float32 quotient, 0..15
 __device__ __forceinline__ uint32_t level(float x, float m, float s) {
   return s > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x - m, s)), 0.f), 15.f) : 0u;
@@ -308,12 +323,16 @@ __device__ __forceinline__ void quantise(const Group<T>& x, const T* from, __hal
   for (int i = 0; i < 4; ++i) {
     uint32_t n[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 8; k += 2) {         // two features an instruction where there is one for two
       const int f = (i >> 1) * 16 + (i & 1) * 4 + (k & 3) + (k >> 2) * 8;
-      const float q = __saturatef((x.at(f) - mf) * inv);                   // of 15 levels
-      const float r = fmaf(q, 15.f, kInt);
-      if (fabsf(fmaf(q, 15.f, kInt - r)) > 0.49999f) near_half |= 1u << f;
-      n[k] = __float_as_uint(r);
+      const float2 y = add2(make_float2(x.at(f), x.at(f + 1)), make_float2(-mf, -mf));
+      const float2 q = make_float2(__saturatef(y.x * inv), __saturatef(y.y * inv));        // of 15 levels
+      const float2 r = fma2(q, make_float2(15.f, 15.f), make_float2(kInt, kInt));
+      const float2 off = fma2(q, make_float2(15.f, 15.f), fma2(r, make_float2(-1.f, -1.f), make_float2(kInt, kInt)));
+      if (fabsf(off.x) > 0.49999f) near_half |= 1u << f;
+      if (fabsf(off.y) > 0.49999f) near_half |= 2u << f;
+      n[k] = __float_as_uint(r.x);
+      n[k + 1] = __float_as_uint(r.y);
     }
     uint32_t byte[4];
 #pragma unroll
@@ -338,15 +357,11 @@ __device__ __forceinline__ uint8_t* block_of(const StoreParams& p, int slot, int
 // bytes become words by exchange between lanes and the warp writes whole sectors; other rows write their bytes one by one.  Rows come in windows of 16; a block that begins in a
 // window and goes on into the next belongs to the first.
 template <typename T>
-__global__ void __launch_bounds__(256) append_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 4) append_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int NG = kv4::groups(p.D), halves = (NG + 1) / 2, lane = threadIdx.x & 31, key = lane & 15;
-  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-  const int64_t per_window = 2ll * p.heads * halves;
-  const int64_t window = task / per_window;
-  const int rest = (int)(task - window * per_window), head = rest / (2 * halves), side = rest / halves & 1, g = (rest % halves) * 2 + (lane >> 4);
-  const int64_t row0 = window * 16;
+  const int NG = kv4::groups(p.D), lane = threadIdx.x, key = lane & 15, head = blockIdx.x, side = threadIdx.y & 1, g = (threadIdx.y >> 1) * 2 + (lane >> 4);
+  const int64_t row0 = (((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * blockDim.z + threadIdx.z) * 16;
   if (row0 >= p.rows) return;
   // rows row0 - 16 .. row0 + 31: bit i of `follows`: row i + 1 goes to the place behind row i's
   auto slot_at = [&](int64_t r) { return r >= 0 && r < p.rows ? p.slots[r] : -1; };
@@ -454,16 +469,13 @@ template <typename T>
 __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int NG = kv4::groups(p.D), halves = (NG + 1) / 2, lane = threadIdx.x & 31;
-  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-  const int64_t per_window = 2ll * p.heads * halves;
-  const int64_t window = task / per_window;
-  const int rest = (int)(task - window * per_window), head = rest / (2 * halves), side = rest / halves & 1, g = (rest % halves) * 2 + (lane >> 4);
+  const int NG = kv4::groups(p.D), lane = threadIdx.x, head = blockIdx.x, side = threadIdx.y & 1, g0 = (threadIdx.y >> 1) * 2, g = g0 + (lane >> 4);
+  const int64_t row0 = (((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * blockDim.z + threadIdx.z) * 16;
   constexpr int kParts = Group<T>::kParts, kPitch = kParts + 1;          // 16-byte pieces of a lane's group, and one to spread the banks
   __shared__ uint4 staged[8][32 * kPitch];
-  uint4* mine = staged[threadIdx.x >> 5];
-  const int64_t row = window * 16 + (lane & 15);
-  if (window * 16 >= p.rows) return;
+  uint4* mine = staged[threadIdx.z * blockDim.y + threadIdx.y];
+  const int64_t row = row0 + (lane & 15);
+  if (row0 >= p.rows) return;
   int slot = row < p.rows && g < NG ? p.slots[row] : -1;
   if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); slot = -1; }
   const unsigned live = __ballot_sync(0xffffffffu, slot >= 0);
@@ -497,11 +509,13 @@ __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
   const float s = __half2float(meta[at]), m = __half2float(meta[p.D / 2 + at]);
   float out[32];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int f = (i >> 3) * 16 + (i & 7);
-    const uint32_t b = pairs[i >> 2] >> 8 * (i & 3);
-    out[f] = fmaf((float)(b & 15u), s, m);
-    out[f + 8] = fmaf((float)(b >> 4 & 15u), s, m);
+  for (int i = 0; i < 16; ++i) {             // a level n in place, at bit e of a word, becomes 2^23 + n 2^e, and n 2^e meets s 2^-e: exactly n s before the one rounding
+    const int f = (i >> 3) * 16 + (i & 7), e = 8 * (i & 1);
+    const uint32_t b = i & 2 ? pairs[i >> 2] >> 16 : pairs[i >> 2];
+    const float2 n = add2(make_float2(__uint_as_float(b & 15u << e | 0x4b000000u), __uint_as_float(b & 240u << e | 0x4b000000u)), make_float2(-8388608.f, -8388608.f));
+    const float2 x = fma2(n, e ? make_float2(s * 0x1p-8f, s * 0x1p-12f) : make_float2(s, s * 0x1p-4f), make_float2(m, m));
+    out[f] = x.x;
+    out[f + 8] = x.y;
   }
 #pragma unroll
   for (int i = 0; i < kParts; ++i) mine[lane * kPitch + i] = Group<T>::part(out, i);
@@ -509,9 +523,9 @@ __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < kParts; ++i) {
-    const int piece = i * 32 + lane, of = piece / kParts, part = piece - of * kParts;      // lane `of` has row window * 16 + of % 16, group g0 + of / 16
+    const int piece = i * 32 + lane, of = piece / kParts, part = piece - of * kParts;      // lane `of` has row row0 + of % 16, group g0 + of / 16
     if (live >> of & 1) {
-      T* to = reinterpret_cast<T*>(side ? p.v : p.k) + (window * 16 + (of & 15)) * (side ? p.v_stride : p.k_stride) + head * p.D + ((rest % halves) * 2 + (of >> 4)) * 32;
+      T* to = reinterpret_cast<T*>(side ? p.v : p.k) + (row0 + (of & 15)) * (side ? p.v_stride : p.k_stride) + head * p.D + (g0 + (of >> 4)) * 32;
       reinterpret_cast<uint4*>(to)[part] = mine[of * kPitch + part];
     }
   }
@@ -532,13 +546,10 @@ template <typename T>
 __global__ void __launch_bounds__(256) append_few_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int NG = kv4::groups(p.D);
-  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 3;
-  const int l8 = threadIdx.x & 7, tile = l8 >> 2, t = l8 & 3;
-  const int64_t per_row = 2ll * p.heads * NG;
-  const int64_t row = task / per_row;
-  const int rest = (int)(task - row * per_row), side = rest / (p.heads * NG), head = rest / NG % p.heads, g = rest % NG;
-  const bool there = row < p.rows;
+  const int l8 = threadIdx.x & 7, tile = l8 >> 2, t = l8 & 3, g = threadIdx.x >> 3, pair = blockIdx.x * blockDim.y + threadIdx.y;
+  const int side = pair >= p.heads, head = pair - (side ? p.heads : 0);
+  const int64_t row = (int64_t)blockIdx.y * blockDim.z + threadIdx.z;
+  const bool there = row < p.rows && pair < 2 * p.heads;
   const int slot = there ? p.slots[row] : -1;
   float2 a = make_float2(0.f, 0.f), b = a;
   if (there) {
@@ -547,12 +558,13 @@ __global__ void __launch_bounds__(256) append_few_kernel(const StoreParams p) {
     b = Pair<T>::load(x + 8);
   }
   float lo = fminf(fminf(a.x, a.y), fminf(b.x, b.y)), hi = fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
+  const unsigned eight = 0xffu << ((threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + threadIdx.x & 24);      // the lanes of this group
   bool odd = a.x != a.x || a.y != a.y || b.x != b.x || b.y != b.y;
 #pragma unroll
   for (int off = 1; off < 8; off <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-    odd = __shfl_xor_sync(0xffffffffu, (int)odd, off) | (int)odd;
+    lo = fminf(lo, __shfl_xor_sync(eight, lo, off));
+    hi = fmaxf(hi, __shfl_xor_sync(eight, hi, off));
+    odd = __shfl_xor_sync(eight, (int)odd, off) | (int)odd;
   }
   if (!there || slot < 0) return;
   if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); return; }
@@ -579,13 +591,10 @@ template <typename T>
 __global__ void __launch_bounds__(256) read_few_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int NG = kv4::groups(p.D);
-  const int64_t task = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 3;
-  const int l8 = threadIdx.x & 7, tile = l8 >> 2, t = l8 & 3;
-  const int64_t per_row = 2ll * p.heads * NG;
-  const int64_t row = task / per_row;
-  if (row >= p.rows) return;
-  const int rest = (int)(task - row * per_row), side = rest / (p.heads * NG), head = rest / NG % p.heads, g = rest % NG;
+  const int l8 = threadIdx.x & 7, tile = l8 >> 2, t = l8 & 3, g = threadIdx.x >> 3, pair = blockIdx.x * blockDim.y + threadIdx.y;
+  const int side = pair >= p.heads, head = pair - (side ? p.heads : 0);
+  const int64_t row = (int64_t)blockIdx.y * blockDim.z + threadIdx.z;
+  if (row >= p.rows || pair >= 2 * p.heads) return;
   const int slot = p.slots[row];
   if (slot < 0) return;
   if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); return; }
@@ -645,14 +654,26 @@ int32_t store_params(const char* who, Ctx* ctx, int32_t dtype, const void* k, co
 }
 
 // Both ways give the same bits.  The wide one has a quarter of the threads, each with four times the work: below kFewGroups groups its chain is longer than what it saves.
+// What a thread has follows from its places in grid and block without a division.
 constexpr int64_t kFewGroups = 24576;
 template <typename K>
 int32_t launch_store(Ctx* ctx, K few, K many, const StoreParams& p) {
   const int NG = kv4::groups(p.D);
-  const bool wide = (int64_t)p.rows * 2 * p.heads * NG > kFewGroups;
-  const int64_t threads = wide ? ceil_div((int64_t)p.rows, 16) * 2 * p.heads * ((NG + 1) / 2) * 32 : (int64_t)p.rows * 2 * p.heads * NG * 8;
-  LMB_REQUIRE(ceil_div(threads, 256) <= INT_MAX, "kv4: %d rows of %d heads are too many for one call", p.rows, p.heads);
-  LMB_CUDA(launch_k_opt(false, wide ? many : few, dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, ctx->stream, p));
+  dim3 grid, block;
+  if ((int64_t)p.rows * 2 * p.heads * NG > kFewGroups) {
+    // warps of a block: sides, pairs of groups, windows; blocks: heads, windows
+    const int per_window = 2 * ((NG + 1) / 2);
+    block = dim3(32, (unsigned)per_window, (unsigned)std::max(1, 8 / per_window));
+    const int64_t blocks = ceil_div(ceil_div((int64_t)p.rows, 16), (int64_t)block.z), y = std::min<int64_t>(blocks, 32768);
+    grid = dim3((unsigned)p.heads, (unsigned)y, (unsigned)ceil_div(blocks, y));
+    LMB_REQUIRE(ceil_div(blocks, y) <= 65535 && (int64_t)p.heads * blocks <= INT_MAX, "kv4: %d rows of %d heads are too many for one call", p.rows, p.heads);
+  } else {
+    // groups of eight lanes of a block: groups of 32 features, heads of both sides, rows
+    const int pairs = std::min(2 * p.heads, 256 / (8 * NG));
+    block = dim3(8u * NG, (unsigned)pairs, (unsigned)std::max(1, std::min(p.rows, 256 / (8 * NG * pairs))));
+    grid = dim3((unsigned)ceil_div(2 * p.heads, pairs), (unsigned)ceil_div(p.rows, (int)block.z));
+  }
+  LMB_CUDA(launch_k_opt(false, (int64_t)p.rows * 2 * p.heads * NG > kFewGroups ? many : few, grid, block, 0, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
 }
