@@ -353,6 +353,8 @@ __device__ __forceinline__ uint8_t* block_of(const StoreParams& p, int slot, int
   return p.pages + (((int64_t)(slot >> p.shift) * p.heads + head) * (1 << (p.shift - 4)) + ((slot & ((1 << p.shift) - 1)) >> 4)) * kv4::block_bytes(p.D);
 }
 
+// Bytes bound it in principle (2 rows in, 0.31 of that out in bf16); what it takes is instructions, of which the exact levels are most, so it wants
+// warps (32768 rows of 8 x 128, both sides, bf16: 53 us, 3.3 TB/s, with five blocks of 256 an SM, 68 with three; float32 71 us, 4.4 TB/s).
 // A warp has 16 rows and two groups of a head's keys or values, a lane a row's 32 features, so the range needs no exchange.  Where 16 neighbouring rows go to the 16 places of a block, their
 // bytes become words by exchange between lanes and the warp writes whole sectors; other rows write their bytes one by one.  Rows come in windows of 16; a block that begins in a
 // window and goes on into the next belongs to the first.
@@ -464,7 +466,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 4) append_kernel(con
   }
 }
 
-// One thread per row, side, head and group: its bytes lie in one run of 32 bytes (keys) or in 8 bytes of each of 8 (values), which the neighbouring keys' threads read too.
+// One thread per row, side, head and group: its bytes lie in one run of 32 bytes (keys) or in 8 bytes of each of 8 (values), which the neighbouring keys' threads read too.  The values go
+// through shared memory, so that a warp writes runs of 128 bytes.  32768 rows of 8 x 128: bf16 41 us, 4.3 TB/s; float32 53 us, 5.9 TB/s.  Slots, bytes and values wait for one another; more rows
+// per warp with the next slots asked for ahead were slower (49 us).
 template <typename T>
 __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
   pdl_launch_dependents();
@@ -480,45 +484,45 @@ __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
   if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); slot = -1; }
   const unsigned live = __ballot_sync(0xffffffffu, slot >= 0);
   if (slot >= 0) {
-  const int key = slot & 15;
-  const uint8_t* block = block_of(p, slot, head);
-  uint32_t pairs[4];                         // as quantise() forms them
-  if (side == 0) {
-    const uint4* src = reinterpret_cast<const uint4*>(block + g * 256 + (key & 7) * 32);
-    const uint4 x = src[0], y = src[1];      // words (t, tile): bytes e = 0 of keys key % 8 and + 8, e = 1
-    const uint32_t pick = key & 8 ? 0x7531 : 0x6420;
-    pairs[0] = __byte_perm(x.x, x.z, pick);
-    pairs[2] = __byte_perm(x.y, x.w, pick);
-    pairs[1] = __byte_perm(y.x, y.z, pick);
-    pairs[3] = __byte_perm(y.y, y.w, pick);
-  } else {
-    const uint8_t* src = block + 8 * p.D + g * 256 + ((key & 7) >> 1) * 8;
-    const int byte = 2 * (key & 1) + (key >> 3);
-    uint2 x[8];
+    const int key = slot & 15;
+    const uint8_t* block = block_of(p, slot, head);
+    uint32_t pairs[4];                         // as quantise() forms them
+    if (side == 0) {
+      const uint4* src = reinterpret_cast<const uint4*>(block + g * 256 + (key & 7) * 32);
+      const uint4 x = src[0], y = src[1];      // words (t, tile): bytes e = 0 of keys key % 8 and + 8, e = 1
+      const uint32_t pick = key & 8 ? 0x7531 : 0x6420;
+      pairs[0] = __byte_perm(x.x, x.z, pick);
+      pairs[2] = __byte_perm(x.y, x.w, pick);
+      pairs[1] = __byte_perm(y.x, y.z, pick);
+      pairs[3] = __byte_perm(y.y, y.w, pick);
+    } else {
+      const uint8_t* src = block + 8 * p.D + g * 256 + ((key & 7) >> 1) * 8;
+      const int byte = 2 * (key & 1) + (key >> 3);
+      uint2 x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const uint2*>(src + j * 32);
-    const uint32_t two = byte | (4 + byte) << 4;
+      for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const uint2*>(src + j * 32);
+      const uint32_t two = byte | (4 + byte) << 4;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      pairs[h] = __byte_perm(__byte_perm(x[4 * h].x, x[4 * h + 1].x, two), __byte_perm(x[4 * h + 2].x, x[4 * h + 3].x, two), 0x5410);
-      pairs[2 + h] = __byte_perm(__byte_perm(x[4 * h].y, x[4 * h + 1].y, two), __byte_perm(x[4 * h + 2].y, x[4 * h + 3].y, two), 0x5410);
+      for (int h = 0; h < 2; ++h) {
+        pairs[h] = __byte_perm(__byte_perm(x[4 * h].x, x[4 * h + 1].x, two), __byte_perm(x[4 * h + 2].x, x[4 * h + 3].x, two), 0x5410);
+        pairs[2 + h] = __byte_perm(__byte_perm(x[4 * h].y, x[4 * h + 1].y, two), __byte_perm(x[4 * h + 2].y, x[4 * h + 3].y, two), 0x5410);
+      }
     }
-  }
-  const __half* meta = reinterpret_cast<const __half*>(block + 16 * p.D) + side * p.D;
-  const int at = side ? kv4::value_meta(key, g) : kv4::key_meta(key, g);
-  const float s = __half2float(meta[at]), m = __half2float(meta[p.D / 2 + at]);
-  float out[32];
+    const __half* meta = reinterpret_cast<const __half*>(block + 16 * p.D) + side * p.D;
+    const int at = side ? kv4::value_meta(key, g) : kv4::key_meta(key, g);
+    const float s = __half2float(meta[at]), m = __half2float(meta[p.D / 2 + at]);
+    float out[32];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {             // a level n in place, at bit e of a word, becomes 2^23 + n 2^e, and n 2^e meets s 2^-e: exactly n s before the one rounding
-    const int f = (i >> 3) * 16 + (i & 7), e = 8 * (i & 1);
-    const uint32_t b = i & 2 ? pairs[i >> 2] >> 16 : pairs[i >> 2];
-    const float2 n = add2(make_float2(__uint_as_float(b & 15u << e | 0x4b000000u), __uint_as_float(b & 240u << e | 0x4b000000u)), make_float2(-8388608.f, -8388608.f));
-    const float2 x = fma2(n, e ? make_float2(s * 0x1p-8f, s * 0x1p-12f) : make_float2(s, s * 0x1p-4f), make_float2(m, m));
-    out[f] = x.x;
-    out[f + 8] = x.y;
-  }
+    for (int i = 0; i < 16; ++i) {             // a level n in place, at bit e of a word, becomes 2^23 + n 2^e, and n 2^e meets s 2^-e: exactly n s before the one rounding
+      const int f = (i >> 3) * 16 + (i & 7), e = 8 * (i & 1);
+      const uint32_t b = i & 2 ? pairs[i >> 2] >> 16 : pairs[i >> 2];
+      const float2 n = add2(make_float2(__uint_as_float(b & 15u << e | 0x4b000000u), __uint_as_float(b & 240u << e | 0x4b000000u)), make_float2(-8388608.f, -8388608.f));
+      const float2 x = fma2(n, e ? make_float2(s * 0x1p-8f, s * 0x1p-12f) : make_float2(s, s * 0x1p-4f), make_float2(m, m));
+      out[f] = x.x;
+      out[f + 8] = x.y;
+    }
 #pragma unroll
-  for (int i = 0; i < kParts; ++i) mine[lane * kPitch + i] = Group<T>::part(out, i);
+    for (int i = 0; i < kParts; ++i) mine[lane * kPitch + i] = Group<T>::part(out, i);
   }
   __syncwarp();
 #pragma unroll
@@ -526,7 +530,7 @@ __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
     const int piece = i * 32 + lane, of = piece / kParts, part = piece - of * kParts;      // lane `of` has row row0 + of % 16, group g0 + of / 16
     if (live >> of & 1) {
       T* to = reinterpret_cast<T*>(side ? p.v : p.k) + (row0 + (of & 15)) * (side ? p.v_stride : p.k_stride) + head * p.D + (g0 + (of >> 4)) * 32;
-      reinterpret_cast<uint4*>(to)[part] = mine[of * kPitch + part];
+      __stcs(reinterpret_cast<uint4*>(to) + part, mine[of * kPitch + part]);
     }
   }
 }
@@ -654,16 +658,17 @@ int32_t store_params(const char* who, Ctx* ctx, int32_t dtype, const void* k, co
 }
 
 // Both ways give the same bits.  The wide one has a quarter of the threads, each with four times the work: below kFewGroups groups its chain is longer than what it saves.
-// What a thread has follows from its places in grid and block without a division.
+// 512 rows of 8 heads of 128 (32768 groups), bf16: append 5.1 as few, 4.7 wide, read 2.9 and 2.4; 256 rows: 3.5 and 4.7, 2.2 and 2.4.  What a thread has follows from its places in
+// grid and block without a division.  The wide blocks have `warps` warps: append 52.5 us with 4 and 54.9 with 8 (32768 rows), read 46 and 43.
 constexpr int64_t kFewGroups = 24576;
 template <typename K>
-int32_t launch_store(Ctx* ctx, K few, K many, const StoreParams& p) {
+int32_t launch_store(Ctx* ctx, K few, K many, int warps, const StoreParams& p) {
   const int NG = kv4::groups(p.D);
   dim3 grid, block;
   if ((int64_t)p.rows * 2 * p.heads * NG > kFewGroups) {
     // warps of a block: sides, pairs of groups, windows; blocks: heads, windows
     const int per_window = 2 * ((NG + 1) / 2);
-    block = dim3(32, (unsigned)per_window, (unsigned)std::max(1, 8 / per_window));
+    block = dim3(32, (unsigned)per_window, (unsigned)std::max(1, warps / per_window));
     const int64_t blocks = ceil_div(ceil_div((int64_t)p.rows, 16), (int64_t)block.z), y = std::min<int64_t>(blocks, 32768);
     grid = dim3((unsigned)p.heads, (unsigned)y, (unsigned)ceil_div(blocks, y));
     LMB_REQUIRE(ceil_div(blocks, y) <= 65535 && (int64_t)p.heads * blocks <= INT_MAX, "kv4: %d rows of %d heads are too many for one call", p.rows, p.heads);
@@ -751,7 +756,7 @@ extern "C" int32_t lmb200_kv4_append(lmb200_ctx h, int32_t dtype, const void* k,
   LMB_TRY(store_params("kv4_append", ctx, dtype, k, v, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
   if (rows == 0) return LMB200_OK;
   LMB_CUDA(cudaSetDevice(ctx->device));
-  return dtype == LMB200_F32 ? launch_store(ctx, append_few_kernel<float>, append_kernel<float>, p) : launch_store(ctx, append_few_kernel<__nv_bfloat16>, append_kernel<__nv_bfloat16>, p);
+  return dtype == LMB200_F32 ? launch_store(ctx, append_few_kernel<float>, append_kernel<float>, 4, p) : launch_store(ctx, append_few_kernel<__nv_bfloat16>, append_kernel<__nv_bfloat16>, 4, p);
 }
 
 extern "C" int32_t lmb200_kv4_read(lmb200_ctx h, int32_t dtype, void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads,
@@ -762,5 +767,5 @@ extern "C" int32_t lmb200_kv4_read(lmb200_ctx h, int32_t dtype, void* k_out, voi
   LMB_TRY(store_params("kv4_read", ctx, dtype, k_out, v_out, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
   if (rows == 0) return LMB200_OK;
   LMB_CUDA(cudaSetDevice(ctx->device));
-  return dtype == LMB200_F32 ? launch_store(ctx, read_few_kernel<float>, read_kernel<float>, p) : launch_store(ctx, read_few_kernel<__nv_bfloat16>, read_kernel<__nv_bfloat16>, p);
+  return dtype == LMB200_F32 ? launch_store(ctx, read_few_kernel<float>, read_kernel<float>, 8, p) : launch_store(ctx, read_few_kernel<__nv_bfloat16>, read_kernel<__nv_bfloat16>, 8, p);
 }
