@@ -36,22 +36,6 @@ def _code(a):
         return _CODES.setdefault(a.dtype, _NAMES.get(str(a.dtype), -1))
 
 
-def _here(device, *arrays):
-    """Refuses arrays of another GPU than the device's: a kernel would fault on them."""
-    for a in arrays:
-        if a is None:
-            continue
-        if isinstance(a, DeviceArray):
-            on = a.device.ordinal
-        else:
-            on = getattr(a, "get_device", None)
-            if on is None:
-                continue
-            on = on()
-        if on >= 0 and on != device.ordinal:               # below 0: host memory, refused by name below
-            raise ValueError(f"an array on GPU {on} for a device on GPU {device.ordinal}")
-
-
 def _count(a):
     try:
         return a.numel()
@@ -59,40 +43,45 @@ def _count(a):
         return math.prod(a.shape)
 
 
-def _address(what, a):
+def _address(what, a, on):
+    """Address of an array on GPU `on`: a kernel would fault on another one's."""
     if isinstance(a, DeviceArray):
-        return a.ptr
-    if not a.is_cuda:
+        gpu, address = a.device.ordinal, a.ptr
+    elif not a.is_cuda:
         raise ValueError(f"{what}: not in device memory")
-    return a.data_ptr()
+    else:
+        gpu, address = a.get_device(), a.data_ptr()
+    if gpu != on:
+        raise ValueError(f"{what}: an array on GPU {gpu} for a device on GPU {on}")
+    return address
 
 
-def _plain(what, a, least):
+def _plain(what, a, least, on):
     """Address of a contiguous array of at least `least` elements."""
     if _count(a) < least:
         raise ValueError(f"{what}: {_count(a)} elements, at least {least} are needed")
     if not isinstance(a, DeviceArray) and not a.is_contiguous():
         raise ValueError(f"{what}: not contiguous")
-    return _address(what, a)
+    return _address(what, a, on)
 
 
-def _ints(what, a, least):
+def _ints(what, a, least, on):
     try:                                       # a step names a dozen of these: torch's own answers first
-        if _CODES[a.dtype] == I32 and a.numel() >= least and a.is_cuda and a.is_contiguous():
+        if _CODES[a.dtype] == I32 and a.numel() >= least and a.get_device() == on and a.is_contiguous():
             return a.data_ptr()
     except (KeyError, AttributeError):
         pass
     if _code(a) != I32:
         raise ValueError(f"{what}: {a.dtype}, expected int32")
-    return _plain(what, a, least)
+    return _plain(what, a, least, on)
 
 
-def _float(what, a):
+def _float(what, a, on):
     """(address, dtype code) of a float32 or bfloat16 array."""
     code = _code(a)
     if code != F32 and code != BF16:
         raise ValueError(f"{what}: {a.dtype}, expected float32 or bfloat16")
-    return _address(what, a), code
+    return _address(what, a, on), code
 
 
 def _rows(what, a, inner):
@@ -124,42 +113,40 @@ def _bytes(a):
     return _count(a) * ((2 if a.dtype == BF16 else 4) if isinstance(a, DeviceArray) else a.element_size())
 
 
-def _pool(pages, page_size, heads, dim):
+def _pool(pages, page_size, heads, dim, on):
     n_pages, shape = pages.shape[0], (page_size, heads, dim)
     each = _PAGE_BYTES.get(shape)
     if each is None:
         each = _PAGE_BYTES[shape] = kv4_page_bytes(*shape)
     if _bytes(pages) < n_pages * each:
         raise ValueError(f"pages: {_bytes(pages)} bytes for {n_pages} pages of {each}")
-    return _plain("pages", pages, 0), n_pages
+    return _plain("pages", pages, 0, on), n_pages
 
 
 def kv_reserve(device, lens, add, table, free_list, n_free, *, page_size, lens_out, n_free_out, cu_rows, slots, status):
     """Pages, slots and lengths for add[b] more tokens of every sequence (lmb200_kv_reserve).  lens_out may be lens, n_free_out n_free."""
-    _here(device, lens, add, table, free_list, n_free, lens_out, n_free_out, cu_rows, slots, status)
-    n, rows = lens.shape[0], slots.shape[0]
-    _call("lmb200_kv_reserve", device.handle, n, page_size, table.shape[1], free_list.shape[0], rows, _ints("lens", lens, n), _ints("add", add, n),
-              _ints("table", table, n * table.shape[1]), _ints("free_list", free_list, 1), _ints("n_free", n_free, 1), _ints("lens_out", lens_out, n),
-              _ints("n_free_out", n_free_out, 1), _ints("cu_rows", cu_rows, n + 1), _ints("slots", slots, 0), _ints("status", status, 1))
+    n, rows, on = lens.shape[0], slots.shape[0], device.ordinal
+    _call("lmb200_kv_reserve", device.handle, n, page_size, table.shape[1], free_list.shape[0], rows, _ints("lens", lens, n, on), _ints("add", add, n, on),
+              _ints("table", table, n * table.shape[1], on), _ints("free_list", free_list, 1, on), _ints("n_free", n_free, 1, on), _ints("lens_out", lens_out, n, on),
+              _ints("n_free_out", n_free_out, 1, on), _ints("cu_rows", cu_rows, n + 1, on), _ints("slots", slots, 0, on), _ints("status", status, 1, on))
 
 
 def kv_shrink(device, lens, drop, table, free_list, n_free, *, page_size, lens_out, n_free_out):
     """The last drop[b] tokens of every sequence leave the cache and their pages go back (lmb200_kv_shrink)."""
-    _here(device, lens, drop, table, free_list, n_free, lens_out, n_free_out)
-    n = lens.shape[0]
-    _call("lmb200_kv_shrink", device.handle, n, page_size, table.shape[1], free_list.shape[0], _ints("lens", lens, n), _ints("drop", drop, n),
-              _ints("table", table, n * table.shape[1]), _ints("free_list", free_list, 1), _ints("n_free", n_free, 1), _ints("lens_out", lens_out, n),
-              _ints("n_free_out", n_free_out, 1))
+    n, on = lens.shape[0], device.ordinal
+    _call("lmb200_kv_shrink", device.handle, n, page_size, table.shape[1], free_list.shape[0], _ints("lens", lens, n, on), _ints("drop", drop, n, on),
+              _ints("table", table, n * table.shape[1], on), _ints("free_list", free_list, 1, on), _ints("n_free", n_free, 1, on), _ints("lens_out", lens_out, n, on),
+              _ints("n_free_out", n_free_out, 1, on))
 
 
 def _store(name, device, k, v, slots, pages, page_size):
-    _here(device, k, v, slots, pages)
     rows, heads, dim = k.shape
-    (kp, code), (vp, v_code) = _float("k", k), _float("v", v)
+    on = device.ordinal
+    (kp, code), (vp, v_code) = _float("k", k, on), _float("v", v, on)
     if code != v_code or v.shape != k.shape:
         raise ValueError(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} differ")
-    pool, n_pages = _pool(pages, page_size, heads, dim)
-    _call(name, device.handle, code, kp, vp, _rows("k", k, heads * dim), _rows("v", v, heads * dim), rows, heads, dim, _ints("slots", slots, rows), pool, n_pages,
+    pool, n_pages = _pool(pages, page_size, heads, dim, on)
+    _call(name, device.handle, code, kp, vp, _rows("k", k, heads * dim), _rows("v", v, heads * dim), rows, heads, dim, _ints("slots", slots, rows, on), pool, n_pages,
               page_size)
 
 
@@ -182,19 +169,18 @@ def kv4_attention_workspace(device, head_dim):
 
 def kv4_attention(device, q, out, cu_rows, lens, table, pages, *, page_size, workspace, scale=None, window=0):
     """Causal attention of the sequences' last tokens, q and out [rows, heads, head_dim], over the cache (lmb200_kv4_attention)."""
-    _here(device, q, out, cu_rows, lens, table, pages, workspace)
     rows, n_heads, dim = q.shape
-    n = lens.shape[0]
-    (qp, code), (op, out_code) = _float("q", q), _float("out", out)
+    n, on = lens.shape[0], device.ordinal
+    (qp, code), (op, out_code) = _float("q", q, on), _float("out", out, on)
     if code != out_code or out.shape != q.shape:
         raise ValueError(f"q {q.dtype} {tuple(q.shape)} and out {out.dtype} {tuple(out.shape)} differ")
     heads = pages.shape[1]
     if n_heads % heads:
         raise ValueError(f"{n_heads} query heads over {heads} kv heads")
-    pool, n_pages = _pool(pages, page_size, heads, dim)
-    _call("lmb200_kv4_attention", device.handle, code, qp, _rows("q", q, n_heads * dim), op, _rows("out", out, n_heads * dim), rows, n, _ints("cu_rows", cu_rows, n + 1),
-              _ints("lens", lens, n), _ints("table", table, n * table.shape[1]), table.shape[1], pool, n_pages, page_size, heads, n_heads // heads, dim,
-              dim ** -0.5 if scale is None else scale, window, _plain("workspace", workspace, 0), _bytes(workspace))
+    pool, n_pages = _pool(pages, page_size, heads, dim, on)
+    _call("lmb200_kv4_attention", device.handle, code, qp, _rows("q", q, n_heads * dim), op, _rows("out", out, n_heads * dim), rows, n, _ints("cu_rows", cu_rows, n + 1, on),
+              _ints("lens", lens, n, on), _ints("table", table, n * table.shape[1], on), table.shape[1], pool, n_pages, page_size, heads, n_heads // heads, dim,
+              dim ** -0.5 if scale is None else scale, window, _plain("workspace", workspace, 0, on), _bytes(workspace))
 
 
 def verify_drafts_workspace(rows):
@@ -207,13 +193,12 @@ def verify_drafts_workspace(rows):
 def verify_drafts(device, target, draft, cu_rows, tokens, temperature, accept_u, sample_u, tokens_out, n_out, drop, *, workspace):
     """Judges drafted tokens by the target's logits [rows, vocab] (lmb200_verify_drafts).  draft: the draft model's logits, or None for drafts that were certain;
     temperature: one per sequence, or None for the largest logit everywhere."""
-    _here(device, target, draft, cu_rows, tokens, temperature, accept_u, sample_u, tokens_out, n_out, drop, workspace)
     rows, vocab = target.shape
-    n = n_out.shape[0]
-    tp, code = _float("target", target)
+    n, on = n_out.shape[0], device.ordinal
+    tp, code = _float("target", target, on)
     dp, d_stride = None, 0
     if draft is not None:
-        dp, d_code = _float("draft", draft)
+        dp, d_code = _float("draft", draft, on)
         if d_code != code or draft.shape != target.shape:
             raise ValueError(f"target {target.dtype} {tuple(target.shape)} and draft {draft.dtype} {tuple(draft.shape)} differ")
         d_stride = _rows("draft", draft, vocab)
@@ -222,12 +207,12 @@ def verify_drafts(device, target, draft, cu_rows, tokens, temperature, accept_u,
         if a is None:
             randoms.append(None)
             continue
-        if _float(what, a)[1] != F32:
+        if _float(what, a, on)[1] != F32:
             raise ValueError(f"{what}: {a.dtype}, expected float32")
-        randoms.append(_plain(what, a, least))
-    _call("lmb200_verify_drafts", device.handle, code, tp, _rows("target", target, vocab), dp, d_stride, vocab, rows, n, _ints("cu_rows", cu_rows, n + 1),
-              _ints("tokens", tokens, rows), *randoms, _ints("tokens_out", tokens_out, rows), _ints("n_out", n_out, n), _ints("drop", drop, n),
-              _plain("workspace", workspace, 0), _bytes(workspace))
+        randoms.append(_plain(what, a, least, on))
+    _call("lmb200_verify_drafts", device.handle, code, tp, _rows("target", target, vocab), dp, d_stride, vocab, rows, n, _ints("cu_rows", cu_rows, n + 1, on),
+              _ints("tokens", tokens, rows, on), *randoms, _ints("tokens_out", tokens_out, rows, on), _ints("n_out", n_out, n, on), _ints("drop", drop, n, on),
+              _plain("workspace", workspace, 0, on), _bytes(workspace))
 
 
 __all__ = ["kv4_page_bytes", "kv_reserve", "kv_shrink", "kv4_append", "kv4_read", "kv4_attention_workspace", "kv4_attention", "verify_drafts_workspace", "verify_drafts"]

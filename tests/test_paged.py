@@ -133,7 +133,7 @@ def test_wrappers_refuse_arrays_that_do_not_fit(lib_built):
     L = lib_built
 
     class Dev:
-        handle = FakeContext().handle
+        handle, ordinal = FakeContext().handle, 0
 
     class Gpu:
         """Looks like a tensor on the GPU."""
@@ -142,6 +142,7 @@ def test_wrappers_refuse_arrays_that_do_not_fit(lib_built):
             self.shape, self.dtype, self.is_cuda, self._c = shape, dtype, True, contiguous
 
         def data_ptr(self): return 256
+        def get_device(self): return 0
         def is_contiguous(self): return self._c
         def element_size(self): return torch.empty(0, dtype=self.dtype).element_size()
 
