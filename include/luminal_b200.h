@@ -631,8 +631,8 @@ int32_t lmb200_kv4_read(lmb200_ctx ctx, int32_t dtype, void* k_out, void* v_out,
                         const int32_t* slots, const void* pages, int32_t n_pages, int32_t page_size);
 /* out = softmax(scale q K^T) V over the cache, causal: the rows of sequence b (cu_rows as above) are its last tokens, each sees itself and every token before it, or
  * the last `window` of them (0: all).  `lens` counts the rows' own tokens, so they are appended first.  q and out: [rows, n_kv_heads * group, head_dim] in dtype, the query
- * heads of a kv head side by side, rows q_stride / out_stride elements apart, each on a 16-byte boundary.  Rows behind cu_rows[n_seq] are left as they are; a row that sees
- * no key is 0.  Scores, softmax and sums in float32.  workspace: lmb200_kv4_attention_workspace bytes, zero before its first use (every call leaves it
+ * heads of a kv head side by side, rows q_stride / out_stride elements apart, each on a 16-byte boundary.  out may be q.  Rows behind cu_rows[n_seq] are left as they are; a row
+ * that sees no key is 0.  Scores, softmax and sums in float32.  workspace: lmb200_kv4_attention_workspace bytes, zero before its first use (every call leaves it
  * usable for the next); calls that may run at the same time need one each. */
 int32_t lmb200_kv4_attention_workspace(lmb200_ctx ctx, int32_t head_dim, int64_t* bytes);
 int32_t lmb200_kv4_attention(lmb200_ctx ctx, int32_t dtype, const void* q, int64_t q_stride, void* out, int64_t out_stride, int32_t rows, int32_t n_seq, const int32_t* cu_rows,

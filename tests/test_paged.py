@@ -971,3 +971,81 @@ def test_append_many_rows(on_torch, dtype, rows, heads, D, page, offset):
     with pytest.raises(L.LuminalB200Error):
         dev.sync()
     assert torch.equal(short[..., :16 * D], before[..., :16 * D])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_over_its_own_queries(on_torch, dtype):
+    """out = q: what is written is read by no one else, in triples that many CTAs share as well."""
+    import torch
+    L, dev = on_torch
+    q, cu, lens, table, pages = one_case(np.random.default_rng(9), dtype, lens=(9000, 300, 5000), new=(9, 1, 3))
+    want, ws = attend(L, dev, q, cuda(cu), cuda(lens), cuda(table), cuda(pages), 16, 0.1)
+    for _ in range(3):
+        own = q.clone()
+        attend(L, dev, own, cuda(cu), cuda(lens), cuda(table), cuda(pages), 16, 0.1, ws=ws, out=own)
+        dev.sync()
+        assert torch.equal(own, want)
+
+
+@pytest.mark.gpu
+def test_attention_of_the_most_sequences(on_torch):
+    """8192 sequences, some of them without rows, some without tokens."""
+    L, dev = on_torch
+    rng = np.random.default_rng(10)
+    lens = rng.integers(0, 40, 8192).astype(np.int32)
+    new = rng.integers(0, 3, 8192)
+    table, n_pages = tables(rng, lens, 16)
+    pages = filled(rng, n_pages, 1, 16, 32)
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    q = cuda(rng.standard_normal((int(cu[-1]), 1, 32)).astype(np.float32))
+    want, size = P.attention(q.cpu().numpy(), cu, lens, table, pages, 16, 0.2)
+    out, _ = attend(L, dev, q, cuda(cu), cuda(lens), cuda(table), cuda(pages), 16, 0.2)
+    dev.sync()
+    check(out, want, size, "f32")
+
+
+@pytest.mark.gpu
+def test_append_and_read_of_millions_of_rows(on_torch):
+    """More windows of rows than one dimension of a grid takes: the same bits as in pieces."""
+    import torch
+    L, dev = on_torch
+    rows, page = 2200011, 256
+    n_pages = -(-rows // page) + 1
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(rows, 1, 32, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    slots = torch.arange(rows, dtype=torch.int32, device="cuda") + 5
+    whole, pieces = (torch.zeros(n_pages, 1, page // 16, 640, dtype=torch.uint8, device="cuda") for _ in range(2))
+    L.kv4_append(dev, k, v, slots, whole, page_size=page)
+    for a in range(0, rows, 100000):
+        L.kv4_append(dev, k[a:a + 100000], v[a:a + 100000], slots[a:a + 100000], pieces, page_size=page)
+    dev.sync()
+    assert torch.equal(whole, pieces)
+    outs = [torch.full_like(k, 9) for _ in range(4)]
+    L.kv4_read(dev, outs[0], outs[1], slots, whole, page_size=page)
+    for a in range(0, rows, 100000):
+        L.kv4_read(dev, outs[2][a:a + 100000], outs[3][a:a + 100000], slots[a:a + 100000], whole, page_size=page)
+    dev.sync()
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+    spread = k.float().amax(-1, keepdim=True) - k.float().amin(-1, keepdim=True)
+    # half a level, 1/30 of the spread; the minimum's and the scale's roundings to halves (2^-12 each of values below 8: 16 roundings at most), and the result's to bf16
+    assert ((outs[0].float() - k.float()).abs() <= spread / 30 + 16 * 8 * 2.0 ** -12 + 8 * 2.0 ** -8).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [None, 1.0])
+def test_verify_the_most_sequences(on_torch, temperature):
+    """65535 sequences of one row each: the largest logit, or for so peaked ones the same by chance."""
+    import torch
+    L, dev = on_torch
+    n, vocab = 65535, 5
+    best = torch.from_numpy(np.random.default_rng(11).integers(0, vocab, n)).cuda()
+    logits = torch.nn.functional.one_hot(best, vocab).float() * 200
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    ints = [torch.full((n,), 7, dtype=torch.int32, device="cuda") for _ in range(4)]
+    u = torch.rand(n, device="cuda")
+    t = None if temperature is None else torch.full((n,), temperature, device="cuda")
+    ws = torch.empty(L.verify_drafts_workspace(n), dtype=torch.uint8, device="cuda")
+    L.verify_drafts(dev, logits, None, cu, ints[0], t, u, u, ints[1], ints[2], ints[3], workspace=ws)
+    dev.sync()
+    assert torch.equal(ints[1].long(), best) and (ints[2] == 1).all() and (ints[3] == 0).all()
