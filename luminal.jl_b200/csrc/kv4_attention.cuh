@@ -12,6 +12,11 @@
 // Work.  Units of 128 keys of all (sequence, row tile, kv head) triples in a row are cut into equal shares whatever the sequences' lengths, so a long sequence among short ones
 // is shared by many CTAs.  Little work is cut into pieces of triples instead, one per CTA, if none becomes much longer than a share: a second triple costs a CTA about 7 us.  Each of a CTA's four warps takes 32 keys of a unit through a ring of bulk copies of its own, which is filled with the next triple's keys while the present
 // one's sums are joined.  Where a triple is cut, its shares leave partial sums and the last one to finish joins them (many: in groups first).
+//
+// What bounds it, in bf16 with 8 kv heads of 128 and 4 query heads each.  32 sequences of 8184 keys: 73 us, 4.6 TB/s, 0.70 of the copy rate; about 300 warp instructions per 16 keys and head,
+// issued at 56 % by 3.3 warps a scheduler that wait for their own arithmetic (three CTAs an SM and more stages: 70 us, but 20 instead of 13.7 for 64 sequences of 300 keys, where a CTA's
+// start is what it takes).  One sequence: 10.4 us for 300 keys, 16 for 8192, 44 for 131072; about 8 of them are the chain of lengths, table, queries, first copy and join.  float32 has three
+// products for one: 32 sequences of 4096 keys 73 us against 42.
 #pragma once
 #include <math_constants.h>
 
