@@ -13,9 +13,8 @@
 // is shared by many CTAs.  Little work is cut into pieces of triples instead, one per CTA, if none becomes much longer than a share: a second triple costs a CTA about 7 us.  Each of a CTA's four warps takes 32 keys of a unit through a ring of bulk copies of its own, which is filled with the next triple's keys while the present
 // one's sums are joined.  Where a triple is cut, its shares leave partial sums and the last one to finish joins them (many: in groups first).
 //
-// What bounds it, in bf16 with 8 kv heads of 128 and 4 query heads each.  32 sequences of 8184 keys: 73 us, 4.6 TB/s, 0.70 of the copy rate; about 300 warp instructions per 16 keys and head,
-// issued at 56 % by 3.3 warps a scheduler that wait for their own arithmetic (three CTAs an SM and more stages: 70 us, but 20 instead of 13.7 for 64 sequences of 300 keys, where a CTA's
-// start is what it takes).  One sequence: 10.4 us for 300 keys, 16 for 8192, 44 for 131072; about 8 of them are the chain of lengths, table, queries, first copy and join.  float32 has three
+// What bounds it, in bf16 with 8 kv heads of 128 and 4 query heads each.  32 sequences of 8184 keys: 70.6 us, 4.8 TB/s, 0.73 of the copy rate; about 300 warp instructions per 16 keys and head,
+// issued at 56 % by 3.3 warps a scheduler that wait for their own arithmetic.  One sequence: 9.6 us for 300 keys, 16 for 8192, 44 for 131072; about 8 of them are the chain of lengths, table, queries, first copy and join.  float32 has three
 // products for one: 32 sequences of 4096 keys 73 us against 42.
 #pragma once
 #include <math_constants.h>
@@ -29,7 +28,9 @@ namespace kv4 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kUnit = 128, kMaxSeqs = 8192;
 constexpr int kCounters = 2048, kMostShares = kCounters / 2, kJoin = 16;
-constexpr unsigned kLonger = 8;                    // units by which a piece may be longer than a share
+// Units by which the longest piece may be longer than a share for the work to be cut into pieces.  As shares and as pieces, us: 64 sequences of 300 keys 22.6 and 13.7, 32 of 1000 24.3 and
+// 18.8 (3 units longer), 20 of 4000 31.1 and 30.4 (4 longer), 16 of 8192 38.7 and 41.2, 32 of 8184 70.6 and 73.0 (5 longer).
+constexpr unsigned kLonger = 4;
 
 struct Params {
   const void* q;
@@ -213,8 +214,9 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
       all = of = 0;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) { all += (unsigned)shared_word[w]; of += (unsigned)shared_word[8 + w]; }
-      if (of < gridDim.x) {
-        const unsigned room = gridDim.x - of, each = max(1u, (all + room - 1) / room);           // sum of ceil(n / each) <= all / each + of <= the CTAs
+      const unsigned room = gridDim.x - min(of, gridDim.x);
+      if (room > 0 && all > room) {          // (else every unit has a CTA)
+        const unsigned each = (all + room - 1) / room;       // sum of ceil(n / each) <= all / each + of <= the CTAs
         unsigned longest = 0, pieces = 0;
         for (int b = b0; b < b1; ++b) {
           if (before[b + 1] == 0) continue;
