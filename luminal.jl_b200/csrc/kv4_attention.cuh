@@ -20,6 +20,7 @@
 #include <math_constants.h>
 
 #include "kv4.cuh"
+#include "kv4_shares.cuh"
 #include "pdl.cuh"
 #include "tc.cuh"
 
@@ -27,7 +28,6 @@ namespace lmb {
 namespace kv4 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kUnit = 128, kMaxSeqs = 8192;
-constexpr int kCounters = 2048, kMostShares = kCounters / 2, kJoin = 16;
 // Units by which the longest piece may be longer than a share for the work to be cut into pieces.  As shares and as pieces, us: 64 sequences of 300 keys 22.6 and 13.7, 32 of 1000 24.3 and
 // 18.8 (3 units longer), 20 of 4000 31.1 and 30.4 (4 longer), 16 of 8192 38.7 and 41.2, 32 of 8184 70.6 and 73.0 (5 longer).
 constexpr unsigned kLonger = 4;
@@ -41,7 +41,7 @@ struct Params {
   const int *cu_rows, *lens, *table;
   const uint8_t* pages;
   int* dev_err;
-  unsigned* counters;                        // [kCounters], zero between calls: per share one for all of a triple's shares and one for a group of them
+  unsigned* counters;                        // [kCounters], zero between calls
   float2* part_ml;                           // [share][2][columns]: maximum (log2) and sum
   float* part_o;                             // [share][2][columns][D]
 };
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
   const int per_page = 1 << (p.shift - 4);
 
   // the next segment of the CTA's share into *sg; false behind the last
-  const int64_t u_end = U * (blockIdx.x + 1) / grid;
+  const int64_t u_end = share_begin((int)blockIdx.x + 1, U, grid);
   auto advance = [&](Segment* sg) __attribute__((always_inline)) -> bool {
     const int64_t u = walk->u;
     if (u >= u_end) return false;
@@ -383,7 +383,6 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
   };
 
   // The last of the shares that cut a triple joins what all of them left; of more than kJoin + kJoin / 2 the last of every kJoin neighbours first joins theirs.
-  struct Part { int first, count, groups, sa; };           // what a part's counter counts: `count` shares from `first` on; groups > 1: of one of so many groups
   auto counted = [&](unsigned* counter, int of) __attribute__((always_inline)) {           // thread 0, behind a barrier behind all threads' writes
     unsigned old;
     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(counter) : "memory");
@@ -392,15 +391,8 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
     shared_word[4] = last;
   };
   auto count_part = [&](const Segment* my) __attribute__((always_inline)) {
-    Part q;
-    q.sa = (int)(((my->item0 + 1) * grid - 1) / U);
-    const int n = (int)(((my->item0 + my->n_pieces) * grid - 1) / U) - q.sa + 1;
-    const bool grouped = n > kJoin + kJoin / 2;
-    const int group = grouped ? ((int)blockIdx.x - q.sa) / kJoin : 0;
-    q.groups = grouped ? (n + kJoin - 1) / kJoin : 1;
-    q.first = q.sa + group * kJoin;
-    q.count = grouped ? min(kJoin, n - group * kJoin) : n;
-    if (tid == 0) counted(p.counters + (grouped ? kMostShares : 0) + q.first, q.count);
+    const Part q = part_of(my->item0, my->n_pieces, (int)blockIdx.x, U, grid);
+    if (tid == 0) counted(p.counters + part_counter(q), q.count);
     return q;
   };
   // behind the barrier behind count_part
@@ -452,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
       }
       __syncthreads();
       if (done) break;
-      if (tid == 0) counted(p.counters + q.sa, q.groups);
+      if (tid == 0) counted(p.counters + triple_counter(q), q.groups);
       __syncthreads();
       if (!shared_word[4]) break;
       first = q.sa;
@@ -462,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
   };
 
   {
-    const int64_t u = U * blockIdx.x / grid;
+    const int64_t u = share_begin((int)blockIdx.x, U, grid);
     int lo = 0, hi = p.n_seq - 1;            // the last sequence with before[b] <= u
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
