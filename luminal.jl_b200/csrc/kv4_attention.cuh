@@ -19,6 +19,8 @@
 #pragma once
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "kv4.cuh"
 #include "kv4_shares.cuh"
 #include "pdl.cuh"
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
   constexpr int D = S::D, COLS = S::COLS, kStages = S::kStages;
   constexpr bool kSplit = S::kSplit;
   constexpr int BK = 2;                      // blocks of 16 keys whose scores are in registers at once
-  constexpr float kPScale = 7.f;             // weights are 2^7 p at the maximum, up to 2^15 while it lags
+  constexpr float kPScale = 7.f, kPMost = 15.f;            // weights are 2^7 p at the maximum, up to 2^15 while it lags
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* at = smem;
   uint8_t* my_ring = at + (threadIdx.x >> 5) * kStages * S::kStageBytes; at += S::kRing;
@@ -531,14 +533,14 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
     for (int nt = 0; nt < NT; ++nt) { cs[nt][0] = col_scale[nt * 8 + 2 * t]; cs[nt][1] = col_scale[nt * 8 + 2 * t + 1]; }
 
     // ---- one pass over the keys ----------------------------------------------------------------------------------------
-    // Weights up to 2^15 times scales above 1 may leave the halves' range.  The quick way does not look; where its sums are no numbers the segment is gone through
-    // again, scales then taken times 2^-r.
+    // Weights times scales are halves, which end at 2^16 and at 2^-24.  The quick way takes them as they are; where its sums are no numbers, or so small that the roundings of
+    // subnormals may show, the segment is gone through again with care: the maximum never lags, and the products of each block, row and group are brought to the top of the halves by a power of
+    // two of their own, so no group, row or key takes bits from another.
     float m[NT][2], l[NT][2], o[2 * NG][NT][4], om[NT][4];
-    int r;
     uint32_t seen;                           // columns that have a maximum; m of the others is 0
     const int n_stages = sg->n_stages, first_key = (sg->first_block + 2 * warp) * 16, all_from = sg->all_from, all_to = sg->all_to;
-    for (bool careful = false;; careful = true) {
-      r = 0;
+    auto pass = [&](auto with_care) __attribute__((always_inline)) {
+      constexpr bool careful = decltype(with_care)::value;
       seen = 0;
       bool ready = false;                    // all columns have one
 #pragma unroll
@@ -672,35 +674,6 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
               odd_values = __any_sync(0xffffffffu, odd_values);
               tc::fence_async_smem();        // before the next copy into this stage
             }
-            if (careful) {
-              __half2 most = __float2half2_rn(0.f);
-              uint32_t* scales = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage) + 576 * NG);
-#pragma unroll
-              for (int kb = 0; kb < BK; ++kb)
-                for (int i = lane; i < 8 * NG; i += 32) {
-                  const uint32_t sc = scales[kb * 160 * NG + i];
-                  most = __hmax2(most, as_half2(sc & ~odd_halves(sc)));
-                }
-              float x = fmaxf(__low2float(most), __high2float(most));
-#pragma unroll
-              for (int off = 16; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-              if (x > __uint_as_float((uint32_t)(127 + r) << 23)) {        // above 2^r: weights up to 2^15 times scales up to 1 stay halves
-                const int rn = (int)(__float_as_uint(x) >> 23) - 126;                      // x < 2^rn
-                const float fade = __uint_as_float((uint32_t)(127 + r - rn) << 23);
-                r = rn;
-#pragma unroll
-                for (int i = 0; i < 2 * NG; ++i)
-#pragma unroll
-                  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[i][nt][k] *= fade;
-              }
-              const __half2 down = __float2half2_rn(__uint_as_float((uint32_t)(127 - r) << 23));
-#pragma unroll
-              for (int kb = 0; kb < BK; ++kb)
-                for (int i = lane; i < 8 * NG; i += 32) scales[kb * 160 * NG + i] = as_u32(__hmul2(as_half2(scales[kb * 160 * NG + i]), down));
-              tc::fence_async_smem();
-            }
             __syncwarp();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -709,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
                 float x = fmaxf(fmaxf(s[0][nt][k], s[0][nt][k + 2]), fmaxf(s[1][nt][k], s[1][nt][k + 2]));
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                const float rise = x - kPScale;
+                const float rise = x - (careful ? kPMost : kPScale);
                 const bool first = !(seen >> (2 * nt + k) & 1);
                 if (first ? x > -CUDART_INF_F : rise > 0.f) {
                   seen |= 1u << (2 * nt + k);
@@ -771,6 +744,51 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
               const uint2 w = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 256 * NG + gr * 256 + lane * 8);
               const uint2 vs = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 576 * NG + gr * 32 + t * 8);        // in the order of the weights' operand
               uint32_t wb[NT][kSplit ? 4 : 2];
+              if (careful) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {            // lane (g, t): row g's weights of keys 2t, 2t + 1, 2t + 8, 2t + 9
+                  float x[4], top = 0.f;
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    float2 e = __half22float2(as_half2(pb[nt][i])), f = __half22float2(as_half2(i ? vs.y : vs.x));
+                    if (kSplit) {
+                      const float2 lo = __half22float2(as_half2(pb[nt][kSplit ? 2 + i : 0]));
+                      e.x += lo.x;
+                      e.y += lo.y;
+                    }
+                    x[2 * i] = e.x * f.x;
+                    x[2 * i + 1] = e.y * f.y;
+                    top = fmaxf(top, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
+                  }
+                  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                  const int e = max((int)(__float_as_uint(top) >> 23), 60);                // less than 2^-66 is nothing
+                  const float up = __uint_as_float((uint32_t)(268 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);       // to [2^14, 2^15), and back
+                  uint32_t hi[2], lo[2] = {0, 0};
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    hi[i] = pack(x[2 * i] * up, x[2 * i + 1] * up);
+                    const float2 f = __half22float2(as_half2(hi[i]));
+                    if (kSplit) lo[i] = pack(fmaf(x[2 * i], up, -f.x), fmaf(x[2 * i + 1], up, -f.y));
+                  }
+                  const float d0 = __shfl_sync(0xffffffffu, down, 8 * t), d1 = __shfl_sync(0xffffffffu, down, 8 * t + 4);              // of rows 2t, 2t + 1
+#pragma unroll
+                  for (int tile = 0; tile < 2; ++tile) {
+                    const uint32_t y = tile ? w.y : w.x;
+                    const uint32_t a0 = numbers<kSplit>(y, 0x000f000fu), a1 = numbers<kSplit>(y, 0x00f000f0u), a2 = numbers<kSplit>(y >> 8, 0x000f000fu),
+                                   a3 = numbers<kSplit>(y >> 8, 0x00f000f0u);
+                    float acc[4];
+                    if (kSplit) mma_split<true>(acc, a0, a1, a2, a3, hi[0], hi[1], lo[0], lo[1]);
+                    else mma_first(acc, a0, a1, a2, a3, hi[0], hi[1]);
+                    float (&to)[4] = o[2 * gr + tile][nt];
+                    to[0] = fmaf(acc[0], d0, to[0]);
+                    to[1] = fmaf(acc[1], d1, to[1]);
+                    to[2] = fmaf(acc[2], d0, to[2]);
+                    to[3] = fmaf(acc[3], d1, to[3]);
+                  }
+                }
+                continue;
+              }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 if (kSplit) {
@@ -806,17 +824,48 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
         if (j + kStages < n_stages) issue(sg, j + kStages, slot);
         slot = slot + 1 == kStages ? 0 : slot + 1;
       }
-
-      float all = 0.f;
+    };
+    pass(std::false_type());
+    float all = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) all = fmaf(o[i][nt][k], 0.f, all);
+      }
+    bool again = all != 0.f;                 // NaN is not 0 either
+    {
+      // A product is off by 2^-26 (2^-25 at most) where it is subnormal, so a sum over k keys of n about 7 by sqrt(k) 2^-23: less than 2^-20 (bf16: 2^-13) of what is not smaller than this.
+      // First each lane's largest sum of four features, then the group's.  (0 is no rounding's work: the key of the largest weight has at least 2^7 2^-24.)
+      const float least = sqrtf(32.f * n_stages) * (kSplit ? 2.f : 0x1p-30f);            // in units of the high numbers, which count 16 times
+      auto largest = [&](int gr, int nt, int k) __attribute__((always_inline)) {
+        return fmaxf(16.f * fmaxf(o[2 * gr][nt][k], o[2 * gr + 1][nt][k]), fmaxf(o[2 * gr][nt][k + 2], o[2 * gr + 1][nt][k + 2]));
+      };
+      bool small = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int i = 0; i < 2 * NG; ++i) all = fmaf(o[i][nt][k], 0.f, all);
-        }
-      if (careful || !__any_sync(0xffffffffu, all != 0.f)) break;          // NaN is not 0 either
+          for (int gr = 0; gr < NG; ++gr) small |= (seen >> (2 * nt + k) & 1) && largest(gr, nt, k) < least;
+      if (__any_sync(0xffffffffu, small)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+              float x = largest(gr, nt, k);
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+              again |= x > 0.f && x < least;
+            }
+      }
+    }
+    if (__any_sync(0xffffffffu, again)) {
       start(sg, page_at(sg, 0), page_at(sg, 1));
+      pass(std::true_type());
     }
 
     // ---- the next segment's keys are asked for while this one's sums become one -------------------------------------------------
@@ -852,7 +901,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + k]);
         fade[nt][k] = m[nt][k] == -CUDART_INF_F ? (l[nt][k] != l[nt][k] ? 1.f : 0.f) : exp2_fast(m[nt][k] - top);
       }
-    const float up_r = __uint_as_float((uint32_t)(127 + (kSplit ? -4 : 20) + r) << 23);  // of 16 n; n takes another 16
+    constexpr float kUp = kSplit ? 0x1p-4f : 0x1p20f;      // of 16 n; n takes another 16
 #pragma unroll
     for (int turn = 0; turn < 2; ++turn) {   // warps 0 and 1 write, 2 and 3 add
       if (warp >> 1 == turn) {
@@ -862,8 +911,8 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
           for (int nt = 0; nt < NT; ++nt) {
             const float b0 = __shfl_sync(0xffffffffu, om[nt][0], (i >> 1) * 4 + t), b1 = __shfl_sync(0xffffffffu, om[nt][1], (i >> 1) * 4 + t);
             float* dst = merge + ((warp & 1) * COLS + nt * 8 + 2 * t) * S::kPitch + 16 * i + g;
-            const float x0 = fmaf(o[i][nt][0], up_r * 16.f, b0) * fade[nt][0], x1 = fmaf(o[i][nt][1], up_r * 16.f, b1) * fade[nt][1];
-            const float x2 = fmaf(o[i][nt][2], up_r, b0) * fade[nt][0], x3 = fmaf(o[i][nt][3], up_r, b1) * fade[nt][1];
+            const float x0 = fmaf(o[i][nt][0], kUp * 16.f, b0) * fade[nt][0], x1 = fmaf(o[i][nt][1], kUp * 16.f, b1) * fade[nt][1];
+            const float x2 = fmaf(o[i][nt][2], kUp, b0) * fade[nt][0], x3 = fmaf(o[i][nt][3], kUp, b1) * fade[nt][1];
             if (turn == 0) {
               dst[0] = x0; dst[S::kPitch] = x1; dst[8] = x2; dst[S::kPitch + 8] = x3;
             } else {
