@@ -59,16 +59,18 @@ int32_t check_device_error(Ctx* ctx) {
   const int code = ctx->dev_err ? *reinterpret_cast<volatile int*>(ctx->dev_err) : 0;
   if (code != 0) {
     *ctx->dev_err = 0;
-    if (code == kv4::kErrPage)
-      return fail(LMB200_EINVAL, "a slot, a block table or a row offset names a place outside its cache or its rows: what it named was left out of the results");
-    if (code == kv4::kErrFree)
-      return fail(LMB200_EINVAL, "kv_shrink: lengths, block tables and free list do not fit together; nothing was given back");
     if (ctx->nccl_comm && ctx->tp_size > 1) ctx->comm_broken = true;
     if (code == 2)
       return fail(LMB200_ETIMEOUT, "a peer rank's signal was invalid (that rank had a wait run out, or the ranks' step counters "
                                    "differ): results of the last call are invalid; call lmb200_comm_resync on every rank");
     return fail(LMB200_ETIMEOUT, "a kernel gave up a bounded wait (mbarrier / flag): results of the last call are invalid%s",
                 ctx->comm_broken ? "; the tensor-parallel ranks are out of step, call lmb200_comm_resync on every rank" : "");
+  }
+  const int arg = ctx->dev_arg ? *reinterpret_cast<volatile int*>(ctx->dev_arg) : 0;
+  if (arg != 0) {
+    *ctx->dev_arg = 0;
+    if (arg == kv4::kErrFree) return fail(LMB200_EINVAL, "kv_shrink: lengths, block tables and free list do not fit together; nothing was given back");
+    return fail(LMB200_EINVAL, "a slot, a block table or a row offset names a place outside its cache or its rows: what it named was left out of the results");
   }
   return LMB200_OK;
 }
@@ -314,12 +316,13 @@ extern "C" int32_t lmb200_init(int32_t device, lmb200_ctx* out) {
     return fail(LMB200_ECUDA, "init: stream creation failed");
   }
   c->stream = c->own_stream;
-  if (cudaHostAlloc((void**)&c->dev_err, sizeof(int), cudaHostAllocMapped) != cudaSuccess) {
+  if (cudaHostAlloc((void**)&c->dev_err, 2 * sizeof(int), cudaHostAllocMapped) != cudaSuccess) {
     cudaStreamDestroy(c->own_stream);
     delete c;
     return fail(LMB200_ECUDA, "init: pinned allocation failed");
   }
-  *c->dev_err = 0;
+  c->dev_arg = c->dev_err + 1;
+  *c->dev_err = *c->dev_arg = 0;
   if (cudaMalloc((void**)&c->dev_broken, sizeof(int)) != cudaSuccess || cudaMemset(c->dev_broken, 0, sizeof(int)) != cudaSuccess) {
     cudaGetLastError();
     cudaFreeHost(c->dev_err);

@@ -48,7 +48,8 @@ struct Ctx {
   cudaStream_t own_stream = nullptr;
   cudaStream_t stream = nullptr;
   int64_t launches = 0;
-  int* dev_err = nullptr;        // mapped pinned word: a kernel whose bounded wait gave up sets it
+  int* dev_err = nullptr;        // mapped pinned word: a kernel whose bounded wait gave up sets it, and kernels that wait end their waits where it is set
+  int* dev_arg = nullptr;        // the word behind it: a kernel that met arguments it left out says so (kv4::kErr*); no kernel reads it
   int* dev_broken = nullptr;     // device word: set with dev_err by a tensor-parallel wait that failed; while it is
                                  // set every signal this rank sends to its peers is marked invalid (see PeerReduce)
   bool comm_broken = false;      // a tensor-parallel step failed: steps are refused until lmb200_comm_resync
@@ -166,7 +167,7 @@ __device__ __forceinline__ float4 peer_load4(const float* p) {
 #endif
 
 Ctx* ctx_from(lmb200_ctx h);
-// LMB200_ETIMEOUT (and clears the flag) if a kernel reported a wait that ran out
+// LMB200_ETIMEOUT (and clears the flag) if a kernel reported a wait that ran out, else LMB200_EINVAL (the same) if one left arguments out
 int32_t check_device_error(Ctx* ctx);
 int32_t nccl_allreduce_f32(Ctx* ctx, void* dptr, int64_t count, cudaStream_t stream);
 

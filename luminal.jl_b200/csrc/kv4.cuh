@@ -20,8 +20,8 @@ namespace kv4 {
 
 constexpr int kGroup = 32;                 // features that share a scale and a minimum
 constexpr int kMostTokens = 1 << 30;       // of a sequence, and rows of a call: sums of two stay below 2^31
-constexpr int kErrPage = 3;                // Ctx::dev_err: a slot or a block table names a place outside the cache, or the rows do not fit together
-constexpr int kErrFree = 4;                // the free list, the lengths and the tables do not fit together
+constexpr int kErrPage = 1;                // Ctx::dev_arg: a slot or a block table names a place outside the cache, or the rows do not fit together
+constexpr int kErrFree = 2;                // the free list, the lengths and the tables do not fit together
 
 __host__ __device__ inline int groups(int D) { return D / kGroup; }
 __host__ __device__ inline int block_bytes(int D) { return 20 * D; }

@@ -81,6 +81,7 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   p.cu_rows = cu_rows; p.lens = lens; p.table = table;
   p.pages = static_cast<const uint8_t*>(pages);
   p.dev_err = ctx->dev_err;
+  p.dev_arg = ctx->dev_arg;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counters = reinterpret_cast<unsigned*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + kv4::kCounters * 4);

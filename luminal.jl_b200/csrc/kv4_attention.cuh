@@ -42,7 +42,7 @@ struct Params {
   float scale;                               // of the scores, times log2(e)
   const int *cu_rows, *lens, *table;
   const uint8_t* pages;
-  int* dev_err;
+  int *dev_err, *dev_arg;
   unsigned* counters;                        // [kCounters], zero between calls
   float2* part_ml;                           // [share][2][columns]: maximum (log2) and sum
   float* part_o;                             // [share][2][columns][D]
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
       sum += n;
       items += triples;
     }
-    if ((bad || broken) && blockIdx.x == 0) atomicExch(p.dev_err, kErrPage);
+    if ((bad || broken) && blockIdx.x == 0) atomicExch(p.dev_arg, kErrPage);
     // units per piece: 1, or so many that every CTA has one piece
     {
       unsigned all = sum, of = items;
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
   };
   auto checked = [&](const Segment* sg, int batch, int page) __attribute__((always_inline)) {
     if ((unsigned)page < (unsigned)p.n_pages) return page;
-    if (place_of(sg, batch) >= 0) atomicExch(p.dev_err, kErrPage);
+    if (place_of(sg, batch) >= 0) atomicExch(p.dev_arg, kErrPage);
     return -1;
   };
   auto issue = [&](const Segment* sg, int j, int s) __attribute__((always_inline)) {

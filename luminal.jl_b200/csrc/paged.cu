@@ -18,7 +18,7 @@ struct TableParams {
   const int *lens, *change, *n_free;
   int *table, *free_list;                    // reserve writes the table, shrink the free list
   int *lens_out, *n_free_out, *cu_rows, *slots, *status;
-  int* dev_err;
+  int* dev_arg;
 };
 
 __device__ __forceinline__ void cluster_sync_all() {
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kTableThreads) shrink_kernel(const TableParams
   }
   if (tid == 0) {
     *p.n_free_out = free_now + n_back;
-    if (bad) atomicExch(p.dev_err, kv4::kErrFree);
+    if (bad) atomicExch(p.dev_arg, kv4::kErrFree);
   }
 }
 
@@ -225,7 +225,7 @@ struct StoreParams {
   int rows, heads, D, shift, n_pages;
   const int* slots;
   uint8_t* pages;
-  int* dev_err;
+  int* dev_arg;
 };
 
 // The 32 features of one group of one row as a lane holds them.
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 4) append_kernel(con
       }
     } else if (live) {
       if (slot >= places) {
-        atomicExch(p.dev_err, kv4::kErrPage);
+        atomicExch(p.dev_arg, kv4::kErrPage);
       } else {
         const int k16 = slot & 15;
         uint8_t* out = block_of(p, slot, head);
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(256) read_kernel(const StoreParams p) {
   const int64_t row = row0 + (lane & 15);
   if (row0 >= p.rows) return;
   int slot = row < p.rows && g < NG ? p.slots[row] : -1;
-  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); slot = -1; }
+  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_arg, kv4::kErrPage); slot = -1; }
   const unsigned live = __ballot_sync(0xffffffffu, slot >= 0);
   if (slot >= 0) {
     const int key = slot & 15;
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(256) append_few_kernel(const StoreParams p) {
     odd = __shfl_xor_sync(eight, (int)odd, off) | (int)odd;
   }
   if (!there || slot < 0) return;
-  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); return; }
+  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_arg, kv4::kErrPage); return; }
   __half m = __float2half_rn(lo), s = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
   if (odd || __hisinf(m) || __hisinf(s) || __hisnan(s)) m = s = __ushort_as_half(0x7fff);   // a group without a 4-bit form reads back as NaN
   const float mf = __half2float(m), sf = __half2float(s);
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(256) read_few_kernel(const StoreParams p) {
   if (row >= p.rows || pair >= 2 * p.heads) return;
   const int slot = p.slots[row];
   if (slot < 0) return;
-  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_err, kv4::kErrPage); return; }
+  if (slot >= p.n_pages << p.shift) { atomicExch(p.dev_arg, kv4::kErrPage); return; }
   const int key = slot & 15;
   const uint8_t* block = block_of(p, slot, head);
   const uint8_t* data = block + (side ? 8 * p.D : 0);
@@ -653,7 +653,7 @@ int32_t store_params(const char* who, Ctx* ctx, int32_t dtype, const void* k, co
   p->rows = rows; p->heads = heads; p->D = D; p->shift = kv4::page_shift(page); p->n_pages = n_pages;
   p->slots = slots;
   p->pages = static_cast<uint8_t*>(const_cast<void*>(pages));
-  p->dev_err = ctx->dev_err;
+  p->dev_arg = ctx->dev_arg;
   return LMB200_OK;
 }
 
@@ -728,7 +728,7 @@ extern "C" int32_t lmb200_kv_reserve(lmb200_ctx h, int32_t n_seq, int32_t page_s
   LMB_REQUIRE(lens && add && table && free_list && n_free && lens_out && n_free_out && cu_rows && status && (slots || rows == 0), "kv_reserve: null pointer");
   LMB_CUDA(cudaSetDevice(ctx->device));
   TableParams p = {n_seq, kv4::page_shift(page_size), max_pages, n_pages, rows, lens, add, n_free, table, const_cast<int32_t*>(free_list),
-                   lens_out, n_free_out, cu_rows, slots, status, ctx->dev_err};
+                   lens_out, n_free_out, cu_rows, slots, status, ctx->dev_arg};
   LMB_CUDA(launch_cluster(reserve_kernel, n_seq <= 512 && rows <= 2048 ? 1 : rows <= 32768 ? 8 : g_most_ctas, (size_t)n_seq * 12, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
@@ -742,7 +742,7 @@ extern "C" int32_t lmb200_kv_shrink(lmb200_ctx h, int32_t n_seq, int32_t page_si
   LMB_REQUIRE(lens && drop && table && free_list && n_free && lens_out && n_free_out, "kv_shrink: null pointer");
   LMB_CUDA(cudaSetDevice(ctx->device));
   TableParams p = {n_seq, kv4::page_shift(page_size), max_pages, n_pages, 0, lens, drop, n_free, const_cast<int32_t*>(table), free_list,
-                   lens_out, n_free_out, nullptr, nullptr, nullptr, ctx->dev_err};
+                   lens_out, n_free_out, nullptr, nullptr, nullptr, ctx->dev_arg};
   LMB_CUDA(launch_cluster(shrink_kernel, n_seq > 512 ? 8 : 1, (size_t)n_seq * 12, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;

@@ -34,7 +34,7 @@ struct VerifyParams {
   const int *cu_rows, *tokens;
   const float *temperature, *accept_u, *sample_u;
   int *tokens_out, *n_out, *drop;
-  int* dev_err;
+  int* dev_arg;
   int chunks;                                // of the vocabulary
   float4* part;                              // [rows][kSplits]: target's maximum and sum (T <= 0: the place of the maximum), draft's
   // of a sequence, at the place of its first row
@@ -416,7 +416,7 @@ __device__ __forceinline__ void no_rows(const VerifyParams& p, int b) {
   if (threadIdx.x) return;
   p.n_out[b] = 0;
   p.drop[b] = 0;
-  if (p.cu_rows[b + 1] != p.cu_rows[b]) atomicExch(p.dev_err, kv4::kErrPage);
+  if (p.cu_rows[b + 1] != p.cu_rows[b]) atomicExch(p.dev_arg, kv4::kErrPage);
 }
 
 // One CTA per sequence.
@@ -740,7 +740,7 @@ extern "C" int32_t lmb200_verify_drafts(lmb200_ctx h, int32_t dtype, const void*
     return LMB200_OK;
   }
   VerifyParams p = {target, draft, target_stride, draft_stride, vocab, rows, n_seq, vocab <= 4096 ? 1 : kSplits, cu_rows, tokens, temperature, accept_u, sample_u,
-                    tokens_out, n_out, drop, ctx->dev_err, (int)std::min<int64_t>(kMostChunks, ceil_div(vocab, kChunk))};
+                    tokens_out, n_out, drop, ctx->dev_arg, (int)std::min<int64_t>(kMostChunks, ceil_div(vocab, kChunk))};
   p.part = static_cast<float4*>(workspace);
   p.total = reinterpret_cast<double2*>(p.part + (int64_t)rows * kSplits);
   p.weight = reinterpret_cast<double*>(p.total + (int64_t)rows * kMostChunks);
