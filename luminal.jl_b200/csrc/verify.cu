@@ -242,7 +242,7 @@ struct Power {
   double slope, top;                         // log2(e) / T
   float least;                               // logits below it count for nothing: less than 2^-900 of the top's
   __device__ __forceinline__ Power(const double* t, float m, double inv_T) : table(t), slope(inv_T * 1.4426950408889634), top(m) {
-    least = (float)fmax(top - 900.0 / slope, -3.4028234e38);
+    least = __double2float_ru(fmax(top - 900.0 / slope, -(double)FLT_MAX));        // upwards, never to a logit below it: the exponent field has no room for that
   }
   __device__ __forceinline__ double operator()(float x) const {
     asm("min.NaN.f32 %0, %0, 0f7f7fffff;" : "+f"(x));                    // +infinity as the largest float; NaN stays, and fails the comparison
