@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
       const int r0 = p.cu_rows[b], r1 = p.cu_rows[b + 1], l = p.lens[b];
       const int len = min(max(l, 0), capacity);
       int T_ = r1 - r0, first;
-      bad |= l != len;
+      if (l != len) { bad = true; T_ = 0; }                // longer than its table, or negative: left out
       if (r0 < 0 || r1 < r0 || r1 > p.rows) { broken = true; T_ = 0; }
       const unsigned triples = T_ > 0 ? (unsigned)row_tiles(T_, p.G, COLS) * p.heads : 0u, n = triples * units_of(T_, len, first);
       seq_len[b] = len;
