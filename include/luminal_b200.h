@@ -604,8 +604,8 @@ int32_t lmb200_decode_attention_noalloc(lmb200_ctx ctx, int32_t dtype, const voi
  * A slot is page * page_size + place in the page.  The places of a cache that no call has written are the caller's (zeros read back as 0).
  *
  * A slot or a table entry outside the cache, lengths beyond the tables and row offsets that do not ascend within the rows touch no memory: such entries and
- * sequences are left out (kv4_attention: their rows stay as they are; of offsets that descend or leave the rows, all sequences are left out), and the next synchronising call
- * returns LMB200_EINVAL.
+ * sequences are left out (kv_reserve: a token whose page is such an entry, of the table or the free list, has slot -1; kv4_attention: their rows stay as they are; of offsets that
+ * descend or leave the rows, all sequences are left out), and the next synchronising call returns LMB200_EINVAL.
  * max_pages * page_size is at most 2^30.
  * ------------------------------------------------------------------------------------------ */
 int32_t lmb200_kv4_page_bytes(int32_t page_size, int32_t n_kv_heads, int32_t head_dim, int64_t* bytes);
@@ -620,7 +620,8 @@ int32_t lmb200_kv_reserve(lmb200_ctx ctx, int32_t n_seq, int32_t page_size, int3
                           int32_t* status);
 /* The last drop[b] tokens of every sequence leave the cache (drop <= 0: none; drop >= lens[b]: all, the sequence has ended): lens_out = max(0, lens - drop), and the pages
  * that no token needs any more go back to the free list in the reverse of the order in which kv_reserve takes them.  lens_out may be lens and n_free_out
- * n_free.  If lengths, tables and list do not fit together nothing is given back and the next synchronising call returns LMB200_EINVAL. */
+ * n_free.  If lengths, tables and list do not fit together, or a page to be given back is none of the cache's, nothing is given back and the next synchronising
+ * call returns LMB200_EINVAL. */
 int32_t lmb200_kv_shrink(lmb200_ctx ctx, int32_t n_seq, int32_t page_size, int32_t max_pages, int32_t n_pages, const int32_t* lens, const int32_t* drop, const int32_t* table,
                          int32_t* free_list, const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out);
 /* Stores k and v [rows, n_kv_heads, head_dim] (dtype F32 or BF16; rows k_stride / v_stride elements apart, each on a 16-byte boundary) at slots [rows]; a row whose slot is

@@ -1,4 +1,5 @@
 // Block tables on the GPU (lmb200_kv_reserve, lmb200_kv_shrink) and the 4-bit cache's store and load (lmb200_kv4_append, lmb200_kv4_read).
+#include <cooperative_groups.h>
 #include <limits.h>
 
 #include <algorithm>
@@ -21,8 +22,11 @@ struct TableParams {
   int* dev_arg;
 };
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 __device__ __forceinline__ int cluster_rank() { int r; asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
 __device__ __forceinline__ int cluster_size() { int r; asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r)); return r; }
@@ -132,9 +136,14 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const TableParam
       }
       seq[i] = r;
     }
+    bool lost = false;                       // pages that are none of the cache's, of the table or the free list: their tokens have no slot
 #pragma unroll
-    for (int i = 0; i < kTogether; ++i)
-      if (seq[i] < p.rows) p.slots[seq[i]] = (unsigned)page[i] < (unsigned)p.n_pages ? (page[i] << p.shift) + (pos[i] & size1) : -1;
+    for (int i = 0; i < kTogether; ++i) {
+      const bool there = (unsigned)page[i] < (unsigned)p.n_pages;
+      if (seq[i] < p.rows) p.slots[seq[i]] = there ? (page[i] << p.shift) + (pos[i] & size1) : -1;
+      lost |= seq[i] < n_rows && !there;
+    }
+    if (lost) atomicExch(p.dev_arg, kv4::kErrPage);
   }
   for (int k0 = warp * 32; k0 < n_new; k0 += kTogether * warps * 32) {
     int id[kTogether];
@@ -168,12 +177,16 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(const TableParam
   }
 }
 
-// The way back.  A sequence's pages go back behind those of the sequences after it, its last page first: the reverse of taking them.
+// The way back.  A sequence's pages go back behind those of the sequences after it, its last page first: the reverse of taking them.  All of them are looked at before any is
+// written, so a table that names a page outside the cache leaves the list as it was.
 __global__ void __launch_bounds__(kTableThreads) shrink_kernel(const TableParams p) {
   extern __shared__ int sm[];
   int* len = sm;
   int* left = len + p.n_seq;
   int* page0 = left + p.n_seq;               // pages that the sequences before it give back
+  __shared__ int lost;                       // some CTA of the cluster found a page outside the cache
+  if (threadIdx.x == 0) lost = 0;
+  if (cluster_size() > 1) cluster_arrive();  // (waited for before anyone writes into another's `lost`)
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, per = (p.n_seq + kTableThreads - 1) / kTableThreads;
@@ -199,15 +212,28 @@ __global__ void __launch_bounds__(kTableThreads) shrink_kernel(const TableParams
       ep += ((len[b] + size1) >> p.shift) - ((left[b] + size1) >> p.shift);
     }
   __syncthreads();
-  const int n_back = bad ? 0 : (int)tp;
-  const int stride = kTableThreads * cluster_size();
-  for (int k = cluster_rank() * kTableThreads + tid; k < n_back; k += stride) {
+  int n_back = bad ? 0 : (int)tp;
+  const int stride = kTableThreads * cluster_size(), k0 = cluster_rank() * kTableThreads + tid;
+  auto page_of = [&](int k) {
     const int b = last_at_most(page0, 0, p.n_seq - 1, k);
-    const int place = ((left[b] + size1) >> p.shift) + (k - page0[b]);
-    // k counts upwards over sequences and places; the list's top is the first of them
-    p.free_list[free_now + (n_back - 1 - k)] = p.table[(int64_t)b * p.max_pages + place];
+    return p.table[(int64_t)b * p.max_pages + ((left[b] + size1) >> p.shift) + (k - page0[b])];
+  };
+  int mine = 0;                              // page k0; mostly the only one
+  bool outside = false;
+  for (int k = k0; k < n_back; k += stride) {
+    const int page = page_of(k);
+    outside |= (unsigned)page >= (unsigned)p.n_pages;
+    if (k == k0) mine = page;
   }
-  if (cluster_size() > 1) cluster_sync_all(); else __syncthreads();
+  outside = __syncthreads_or(outside);
+  if (cluster_size() > 1) {
+    cluster_wait();
+    if (outside && tid < cluster_size()) *cooperative_groups::this_cluster().map_shared_rank(&lost, tid) = 1;
+    cluster_sync_all();                      // lens and n_free are read by no one any more
+    outside = lost;
+  }
+  if (outside) { bad = 1; n_back = 0; }
+  for (int k = k0; k < n_back; k += stride) p.free_list[free_now + (n_back - 1 - k)] = k == k0 ? mine : page_of(k);      // k counts upwards over sequences and places; the list's top is the first
   if (cluster_rank() != 0) return;
   for (int b = tid; b < p.n_seq; b += kTableThreads) {
     if (!bad) p.lens_out[b] = left[b];
