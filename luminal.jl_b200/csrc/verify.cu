@@ -5,7 +5,7 @@
 // the smallest j with sum_{i <= j} w_i > u' sum w, w = max(p - q, 0), and w = p behind the last draft.  T <= 0: the largest logit judges and is given.
 //
 // Launches.  statistics_kernel reads every row once, split over CTAs, and leaves a maximum and a sum per part; decide_kernel joins the parts and finds the row that gives the token.
-// That row is read again (it is in L2) with everything in 64 bits: where two borders of the running sum lie 1e-6 apart, sums of 32-bit exponentials, off by about 1e-8 of
+// That row is read again (it is in L2) with everything in 64 bits (exp64.cuh): where two borders of the running sum lie 1e-6 apart, sums of 32-bit exponentials, off by about 1e-8 of
 // the total, would now and then choose the neighbour of the right token.  totals_kernel sums its exponentials over chunks of the vocabulary, weights_kernel the weights where they need
 // those totals (max(p - q, 0)), and choose_kernel finds the chunk and in it the token.  at_once_kernel does the last four in one launch with a cluster per sequence: quicker for
 // small vocabularies, slower for large ones, of which an SM gets two sequences or none.
@@ -16,6 +16,7 @@
 
 #include <algorithm>
 
+#include "exp64.cuh"
 #include "kv4.cuh"
 #include "pdl.cuh"
 
@@ -236,27 +237,6 @@ struct Choice {
   float top, draft_top;
 };
 
-// exp((x - top) / T) in 64 bits for a logit x <= top: 2^(k / 32) from a table, times a polynomial of 2^f, |f| <= 1 / 64 (its first term left out is 3e-15).
-struct Power {
-  const double* table;                       // [32] in shared memory: 2^(k / 32)
-  double slope, top;                         // log2(e) / T
-  float least;                               // logits below it count for nothing: less than 2^-900 of the top's
-  __device__ __forceinline__ Power(const double* t, float m, double inv_T) : table(t), slope(inv_T * 1.4426950408889634), top(m) {
-    least = __double2float_ru(fmax(top - 900.0 / slope, -(double)FLT_MAX));        // upwards, never to a logit below it: the exponent field has no room for that
-  }
-  __device__ __forceinline__ double operator()(float x) const {
-    asm("min.NaN.f32 %0, %0, 0f7f7fffff;" : "+f"(x));                    // +infinity as the largest float; NaN stays, and fails the comparison
-    if (!(x >= least)) return 0.0;
-    constexpr double kInt = 6755399441055744.0;                          // 1.5 2^52: a small number added to it leaves its rint in the low bits
-    const double y = ((double)x - top) * slope, shifted = fma(y, 32.0, kInt), f = fma(shifted - kInt, -0.03125, y);
-    const int k = __double2loint(shifted);
-    // ln(2)^n / n!
-    const double e = fma(fma(fma(fma(fma(f, 1.3333558146428443e-3, 9.618129107628477e-3), f, 5.550410866482158e-2), f, 0.24022650695910072), f, 0.6931471805599453), f, 1.0) *
-                     table[k & 31];
-    return __hiloint2double(__double2hiint(e) + (k >> 5) * 1048576, __double2loint(e));
-  }
-};
-
 // A chunk of the chosen row: thread's runs of N neighbouring logits, of the target and the draft.
 template <typename T> struct Chunk {
   static constexpr int N = Run<T>::N;
@@ -322,9 +302,6 @@ __device__ __forceinline__ int first_row(const VerifyParams& p, int b) {
   return r0 < 0 || r1 > p.rows || r1 <= r0 ? -1 : r0;
 }
 __device__ __forceinline__ double inverse_T(const VerifyParams& p, int b) { return fmin(fmax(1.0 / (double)p.temperature[b], 1e-30), 1e30); }
-__device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
-}
 
 // A block finds out which drafts of sequence b (rows r0 to r1 - 1) are taken, and what the next token is chosen from (by all threads known at the end); `writes`: and writes
 // down what is known.  A warp per row.

@@ -40,3 +40,73 @@ def test_verify_logits_one_step_apart_at_temperatures_near_0(on_torch, vocab, dr
     for got, w in zip((out, n_out, drop), want):
         assert np.array_equal(got.cpu().numpy(), w)
     assert (want[0] >= 0).sum() >= n and (want[1] == np.where(np.arange(n) % 2 == 0, 2, 1)).all()
+
+
+# Logits below a top one at many temperatures: this exponential, CUDA's, and how far apart they may be.
+EXP64 = r"""
+#include <cmath>
+#include <cstdio>
+#include <random>
+#include <vector>
+#include "exp64.cuh"
+__global__ void both(const float* x, const float* top, const double* inv_T, double* ours, double* cudas, int n) {
+  __shared__ double table[32];
+  lmb::fill_table(table);
+  __syncthreads();
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+    ours[i] = lmb::Power(table, top[i], inv_T[i])(x[i]);
+    cudas[i] = exp(((double)fminf(x[i], 3.402823466e38f) - (double)top[i]) * inv_T[i]);
+  }
+}
+int main() {
+  const int n = 1 << 22;
+  std::mt19937_64 rng(3);
+  std::uniform_real_distribution<double> u(0, 1);
+  std::vector<float> x(n), top(n);
+  std::vector<double> inv(n), ours(n), cudas(n);
+  for (int i = 0; i < n; ++i) {
+    inv[i] = std::exp2(40 * u(rng) - 20);
+    top[i] = (float)((2 * u(rng) - 1) * std::exp2(20 * u(rng) - 8));
+    const double y = i % 4 == 0 ? -640 * u(rng) : i % 4 == 1 ? -u(rng) : i % 4 == 2 ? -30 * u(rng) : -std::exp2(-50 * u(rng));
+    x[i] = std::fmin(top[i], (float)(top[i] + y / inv[i]));
+  }
+  x[0] = top[0]; x[1] = -INFINITY; x[2] = NAN; x[3] = INFINITY; top[3] = 3.402823466e38f; x[4] = -3.402823466e38f; top[4] = x[4];
+  float *dx, *dt; double *di, *da, *db;
+  cudaMalloc(&dx, n * 4); cudaMalloc(&dt, n * 4); cudaMalloc(&di, n * 8); cudaMalloc(&da, n * 8); cudaMalloc(&db, n * 8);
+  cudaMemcpy(dx, x.data(), n * 4, cudaMemcpyHostToDevice);
+  cudaMemcpy(dt, top.data(), n * 4, cudaMemcpyHostToDevice);
+  cudaMemcpy(di, inv.data(), n * 8, cudaMemcpyHostToDevice);
+  both<<<512, 256>>>(dx, dt, di, da, db, n);
+  cudaMemcpy(ours.data(), da, n * 8, cudaMemcpyDeviceToHost);
+  cudaMemcpy(cudas.data(), db, n * 8, cudaMemcpyDeviceToHost);
+  if (cudaDeviceSynchronize() != cudaSuccess) return printf("%s\n", cudaGetErrorString(cudaGetLastError())), 1;
+  if (ours[0] != 1 || ours[1] != 0 || ours[2] != 0 || ours[3] != 1 || ours[4] != 1) return printf("edges: %g %g %g %g %g\n", ours[0], ours[1], ours[2], ours[3], ours[4]), 1;
+  int counted = 0;
+  double worst = 0;
+  const double half = std::exp2(-53.0);
+  for (int i = 5; i < n; ++i) {
+    const double y = std::fabs((x[i] - (double)top[i]) * inv[i]);               // in units of e
+    if (y > 620) continue;                                                       // 2^-895: nearly all that counts
+    // this one's 2.2e-15 + 6 + 3 |y| roundings, and CUDA's own: its argument's two, its result's one unit in the last place
+    const double limit = 2.3e-15 + (6 + 2 + 5 * y) * half, off = std::fabs(ours[i] / cudas[i] - 1);
+    worst = std::fmax(worst, off / limit);
+    ++counted;
+    if (!(off <= limit)) return printf("x %.9g top %.9g 1/T %.17g: %.17g, CUDA %.17g\n", x[i], top[i], inv[i], ours[i], cudas[i]), 1;
+  }
+  printf("%d compared, at most %.2f of the limit\n", counted, worst);
+  return counted < n / 2;
+}
+"""
+
+
+@pytest.mark.gpu
+def test_the_exponential_beside_cudas(lib_built, device, tmp_path):
+    import os
+    import subprocess
+    from importlib import import_module
+    build = import_module("luminal_jl_b200._build")
+    (tmp_path / "exp64.cu").write_text(EXP64)
+    subprocess.run([build._nvcc(), *build.NVCC_FLAGS, "-I", build.CSRC, str(tmp_path / "exp64.cu"), "-o", str(tmp_path / "exp64")], check=True)
+    r = subprocess.run([str(tmp_path / "exp64")], capture_output=True, text=True, timeout=300, env={**os.environ})
+    print(r.stdout)
+    assert r.returncode == 0, r.stdout + r.stderr
