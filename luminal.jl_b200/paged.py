@@ -2,7 +2,7 @@
 include/luminal_b200.h, where the formats and rules stand.
 
 Arrays are device memory of the caller, as DeviceArrays or as anything with `data_ptr()` and `shape` (torch tensors); a DeviceArray of int32 is one of dtype I32, and a cache is any
-array whose first axis counts its pages.  Calls are asynchronous on the device's stream: `device.set_stream(...)` puts them on the stream that made the arrays (1: the
+array whose first axis counts its pages (of three axes or more the second counts kv heads).  Calls are asynchronous on the device's stream: `device.set_stream(...)` puts them on the stream that made the arrays (1: the
 legacy default stream)."""
 from __future__ import annotations
 
@@ -123,6 +123,16 @@ def _pool(pages, page_size, heads, dim, on):
     return _plain("pages", pages, 0, on), n_pages
 
 
+def _kv_heads(pages, page_size, dim):
+    """kv heads of a cache [pages, kv heads, ...], or [pages, bytes of a page in any dtype]."""
+    if len(pages.shape) > 2:
+        return pages.shape[1]
+    head, held = kv4_page_bytes(page_size, 1, dim), _bytes(pages) // max(1, pages.shape[0])
+    if held < head or held % head:
+        raise ValueError(f"pages: {held} bytes a page are no number of kv heads of {head}")
+    return held // head
+
+
 def kv_reserve(device, lens, add, table, free_list, n_free, *, page_size, lens_out, n_free_out, cu_rows, slots, status):
     """Pages, slots and lengths for add[b] more tokens of every sequence (lmb200_kv_reserve).  lens_out may be lens, n_free_out n_free."""
     n, rows, on = lens.shape[0], slots.shape[0], device.ordinal
@@ -174,7 +184,7 @@ def kv4_attention(device, q, out, cu_rows, lens, table, pages, *, page_size, wor
     (qp, code), (op, out_code) = _float("q", q, on), _float("out", out, on)
     if code != out_code or out.shape != q.shape:
         raise ValueError(f"q {q.dtype} {tuple(q.shape)} and out {out.dtype} {tuple(out.shape)} differ")
-    heads = pages.shape[1]
+    heads = _kv_heads(pages, page_size, dim)
     if n_heads % heads:
         raise ValueError(f"{n_heads} query heads over {heads} kv heads")
     pool, n_pages = _pool(pages, page_size, heads, dim, on)
