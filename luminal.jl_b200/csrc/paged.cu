@@ -704,6 +704,7 @@ int32_t launch_store(Ctx* ctx, K few, K many, int warps, const StoreParams& p) {
     block = dim3(8u * NG, (unsigned)pairs, (unsigned)std::max(1, std::min(p.rows, 256 / (8 * NG * pairs))));
     grid = dim3((unsigned)ceil_div(2 * p.heads, pairs), (unsigned)ceil_div(p.rows, (int)block.z));
   }
+  LMB_CUDA(cudaSetDevice(ctx->device));
   LMB_CUDA(launch_k_opt(false, (int64_t)p.rows * 2 * p.heads * NG > kFewGroups ? many : few, grid, block, 0, ctx->stream, p));
   ctx->launches++;
   return LMB200_OK;
@@ -781,7 +782,6 @@ extern "C" int32_t lmb200_kv4_append(lmb200_ctx h, int32_t dtype, const void* k,
   StoreParams p;
   LMB_TRY(store_params("kv4_append", ctx, dtype, k, v, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
   if (rows == 0) return LMB200_OK;
-  LMB_CUDA(cudaSetDevice(ctx->device));
   return dtype == LMB200_F32 ? launch_store(ctx, append_few_kernel<float>, append_kernel<float>, 4, p) : launch_store(ctx, append_few_kernel<__nv_bfloat16>, append_kernel<__nv_bfloat16>, 4, p);
 }
 
@@ -792,6 +792,5 @@ extern "C" int32_t lmb200_kv4_read(lmb200_ctx h, int32_t dtype, void* k_out, voi
   StoreParams p;
   LMB_TRY(store_params("kv4_read", ctx, dtype, k_out, v_out, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
   if (rows == 0) return LMB200_OK;
-  LMB_CUDA(cudaSetDevice(ctx->device));
   return dtype == LMB200_F32 ? launch_store(ctx, read_few_kernel<float>, read_kernel<float>, 8, p) : launch_store(ctx, read_few_kernel<__nv_bfloat16>, read_kernel<__nv_bfloat16>, 8, p);
 }
