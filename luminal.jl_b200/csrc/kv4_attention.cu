@@ -49,7 +49,7 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   LMB_REQUIRE(rows >= 0 && n_seq >= 1 && n_seq <= 8192 && window >= 0, "kv4_attention: %d rows, %d sequences (1 to 8192), window %d", rows, n_seq, window);
   const int64_t capacity = (int64_t)max_pages * page_size;
   LMB_REQUIRE(max_pages >= 1 && capacity <= kv4::kMostTokens, "kv4_attention: block tables of %d pages (up to 2^30 tokens)", max_pages);
-  LMB_REQUIRE(rows <= kv4::kMostTokens && (int64_t)rows * group <= INT32_MAX, "kv4_attention: %d rows for each of %d heads", rows, group);
+  LMB_REQUIRE(rows <= kv4::kMostTokens && (int64_t)rows * group <= INT32_MAX - 8 * kv4::kMostTiles, "kv4_attention: %d rows for each of %d heads", rows, group);     // rounded up to tiles in 32 bits
   LMB_REQUIRE(rows == 0 || (q && out && cu_rows && lens && table && pages && workspace), "kv4_attention: null pointer");
   const int64_t width = (int64_t)n_kv_heads * group * head_dim;
   LMB_REQUIRE(q_stride >= width && out_stride >= width, "kv4_attention: row strides %lld and %lld for rows of %lld elements", (long long)q_stride, (long long)out_stride,

@@ -78,3 +78,10 @@ def test_wrappers(lib_built, monkeypatch):
     T.test_wrappers_refuse_arrays_that_do_not_fit(lib_built)
     T.test_wrappers_refuse_arrays_of_another_gpu(lib_built)
     assert not [s for s in said if "context" in s or "CUDA" in s], said
+
+
+@pytest.mark.parametrize("change", [dict(rows=(1 << 30) - 1, group=2), dict(rows=(1 << 30) - 7, group=2), dict(rows=2147483645 // 5, group=5, q_stride=1280, out_stride=1280)])
+def test_attention_rows_whose_tiles_leave_32_bits(lib_built, change):
+    """Rows times query heads fit 32 bits, rounded up to tiles of 8 or 16 they do not."""
+    assert change["rows"] * change["group"] < 2 ** 31
+    assert "rows for each of" in refused(lib_built, "lmb200_kv4_attention", *T._args(heads=1, max_pages=1, **change))
