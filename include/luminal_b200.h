@@ -628,12 +628,12 @@ int32_t lmb200_kv_shrink(lmb200_ctx ctx, int32_t n_seq, int32_t page_size, int32
  * negative is skipped.  No two rows may have the same slot. */
 int32_t lmb200_kv4_append(lmb200_ctx ctx, int32_t dtype, const void* k, const void* v, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads,
                           int32_t head_dim, const int32_t* slots, void* pages, int32_t n_pages, int32_t page_size);
-/* The values that the cache holds at slots [rows], into k_out and v_out; rows whose slot is negative are left as they are. */
+/* The values that the cache holds at slots [rows], into k_out and v_out, which share no memory; rows whose slot is negative are left as they are. */
 int32_t lmb200_kv4_read(lmb200_ctx ctx, int32_t dtype, void* k_out, void* v_out, int64_t k_stride, int64_t v_stride, int32_t rows, int32_t n_kv_heads, int32_t head_dim,
                         const int32_t* slots, const void* pages, int32_t n_pages, int32_t page_size);
 /* out = softmax(scale q K^T) V over the cache, causal: the rows of sequence b (cu_rows as above) are its last tokens, each sees itself and every token before it, or
  * the last `window` of them (0: all).  `lens` counts the rows' own tokens, so they are appended first.  q and out: [rows, n_kv_heads * group, head_dim] in dtype, the query
- * heads of a kv head side by side, rows q_stride / out_stride elements apart, each on a 16-byte boundary.  out may be q.  Rows behind cu_rows[n_seq] are left as they are; a row
+ * heads of a kv head side by side, rows q_stride / out_stride elements apart, each on a 16-byte boundary.  out may be q (with its stride), but not lie over it in part.  Rows behind cu_rows[n_seq] are left as they are; a row
  * that sees no key is 0.  Scores, softmax and sums in float32.  workspace: lmb200_kv4_attention_workspace bytes, zero before its first use (every call leaves it
  * usable for the next); calls that may run at the same time need one each. */
 int32_t lmb200_kv4_attention_workspace(lmb200_ctx ctx, int32_t head_dim, int64_t* bytes);

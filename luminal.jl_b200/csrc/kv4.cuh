@@ -48,5 +48,14 @@ inline int32_t check_cache(const char* who, int n_kv_heads, int D, int n_pages, 
   return LMB200_OK;
 }
 
+// Whether rows of `width` bytes, a_stride and b_stride bytes apart from a and b on, share no byte: arrays apart, or interleaved in the rows of one.
+inline bool apart(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int rows, int64_t width) {
+  const int64_t off = (int64_t)((uintptr_t)b - (uintptr_t)a);
+  if (off >= (rows - 1) * a_stride + width || -off >= (rows - 1) * b_stride + width) return true;
+  if (rows == 1 || a_stride != b_stride) return false;
+  const int64_t in = (off % a_stride + a_stride) % a_stride;
+  return in >= width && in + width <= a_stride;
+}
+
 }  // namespace kv4
 }  // namespace lmb

@@ -57,6 +57,9 @@ extern "C" int32_t lmb200_kv4_attention(lmb200_ctx h, int32_t dtype, const void*
   const int vec = dtype == LMB200_F32 ? 4 : 8;
   LMB_REQUIRE(q_stride % vec == 0 && out_stride % vec == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)pages % 16 == 0 &&
                   (uintptr_t)workspace % 16 == 0, "kv4_attention: rows, pages and workspace must start on 16-byte boundaries");
+  const int64_t size = dtype == LMB200_F32 ? 4 : 2;
+  LMB_REQUIRE(rows == 0 || (out == q && (out_stride == q_stride || rows == 1)) || kv4::apart(q, q_stride * size, out, out_stride * size, rows, width * size),
+              "kv4_attention: out lies over q in part: it may be q with q's stride, or share no byte with it");
   const int64_t need = workspace_bytes_of(ctx, head_dim);
   LMB_REQUIRE(workspace_bytes >= need, "kv4_attention: a workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
   if (rows == 0) return LMB200_OK;

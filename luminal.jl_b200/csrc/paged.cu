@@ -792,5 +792,7 @@ extern "C" int32_t lmb200_kv4_read(lmb200_ctx h, int32_t dtype, void* k_out, voi
   StoreParams p;
   LMB_TRY(store_params("kv4_read", ctx, dtype, k_out, v_out, k_stride, v_stride, rows, n_kv_heads, head_dim, slots, pages, n_pages, page_size, &p));
   if (rows == 0) return LMB200_OK;
+  const int64_t size = dtype == LMB200_F32 ? 4 : 2;
+  LMB_REQUIRE(kv4::apart(k_out, k_stride * size, v_out, v_stride * size, rows, (int64_t)n_kv_heads * head_dim * size), "kv4_read: k_out and v_out share memory");
   return dtype == LMB200_F32 ? launch_store(ctx, read_few_kernel<float>, read_kernel<float>, 8, p) : launch_store(ctx, read_few_kernel<__nv_bfloat16>, read_kernel<__nv_bfloat16>, 8, p);
 }

@@ -1,11 +1,11 @@
 """The refusals of the paged 4-bit cache's operators, each by the check that is meant: with a context that stays alive through the call, so none is refused for its handle."""
-import ctypes as C
 from importlib import import_module
 
 import numpy as np
 import pytest
 
 import test_paged as T
+from test_paged import on_torch  # noqa: F401  (a fixture)
 
 
 class Context(T.FakeContext):
@@ -85,3 +85,45 @@ def test_attention_rows_whose_tiles_leave_32_bits(lib_built, change):
     """Rows times query heads fit 32 bits, rounded up to tiles of 8 or 16 they do not."""
     assert change["rows"] * change["group"] < 2 ** 31
     assert "rows for each of" in refused(lib_built, "lmb200_kv4_attention", *T._args(heads=1, max_pages=1, **change))
+
+
+# rows of 512 elements of 2 bytes
+@pytest.mark.parametrize("change", [dict(out_stride=1024), dict(out_stride=520), dict(out=4096 + 16), dict(out=4096 - 1008), dict(out=4096 + 1024), dict(out=4096 + 1040, q_stride=1000, out_stride=1000),
+                                    dict(out=4096 + 2 * 1024, out_stride=1024), dict(rows=1, out=4096 + 512)])
+def test_attention_out_over_q_in_part(lib_built, change):
+    assert "lies over q" in refused(lib_built, "lmb200_kv4_attention", *T._args(**{**dict(q=4096, out=4096, rows=3), **change}))
+
+
+@pytest.mark.parametrize("change", [dict(v=4096), dict(v=4096 + 256), dict(v=4096 + 768), dict(vs=512), dict(rows=1, v=4096 + 16), dict(v=4096 + 496, ks=500 + 4, vs=500 + 4)])
+def test_read_into_the_same_memory(lib_built, change):
+    a = dict(dtype=1, k=4096, v=4096, ks=256, vs=256, rows=3, heads=4, D=64, slots=256, pages=256, n_pages=9, page=16)
+    a.update(change)
+    assert "share memory" in refused(lib_built, "lmb200_kv4_read", *a.values())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_side_by_side_in_one_array(on_torch, dtype):
+    """q and out, keys and values as columns of the rows of one array, and one behind the other: the bits of arrays of their own."""
+    import torch
+    L, dev = on_torch
+    q, cu, lens, table, pages = T.one_case(np.random.default_rng(60), dtype, lens=(70, 300), new=(2, 4))
+    args = T.cuda(cu), T.cuda(lens), T.cuda(table), T.cuda(pages)
+    want, ws = T.attend(L, dev, q, *args, 16, 0.1)
+    n = q[0].numel()
+    for first, second in ((0, n), (n, 0), (8, n + 16)):
+        both = torch.zeros(len(q), 2 * n + 64, dtype=q.dtype, device="cuda")
+        a, b = (both[:, i:i + n].unflatten(1, q.shape[1:]) for i in (first, second))
+        a.copy_(q)
+        T.attend(L, dev, a, *args, 16, 0.1, ws=ws, out=b)
+        dev.sync()
+        assert torch.equal(b, want) and torch.equal(a, q)
+    both = torch.cat([q, torch.zeros_like(q)])
+    T.attend(L, dev, both[:len(q)], *args, 16, 0.1, ws=ws, out=both[len(q):])
+    slots = T.cuda(np.r_[0:20].astype(np.int32))
+    k, v = (torch.zeros(20, 2, 128, dtype=q.dtype, device="cuda") for _ in range(2))
+    L.kv4_read(dev, k, v, slots, args[3], page_size=16)
+    kv = torch.zeros(20, 4, 128, dtype=q.dtype, device="cuda")
+    L.kv4_read(dev, kv[:, 2:], kv[:, :2], slots, args[3], page_size=16)
+    dev.sync()
+    assert torch.equal(both[len(q):], want) and torch.equal(kv[:, 2:], k) and torch.equal(kv[:, :2], v)
