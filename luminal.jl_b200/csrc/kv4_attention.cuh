@@ -537,14 +537,16 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
     // subnormals may show, the segment is gone through again with care: the maximum never lags, and the products of each block, row and group are brought to the top of the halves by a power of
     // two of their own, so no group, row or key takes bits from another.
     float m[NT][2], l[NT][2], o[2 * NG][NT][4], om[NT][4];
-    uint32_t seen;                           // columns that have a maximum; m of the others is 0
+    uint32_t seen = 0;                       // columns that have a maximum; m of the others is 0
     const int n_stages = sg->n_stages, first_key = (sg->first_block + 2 * warp) * 16, all_from = sg->all_from, all_to = sg->all_to;
-    auto pass = [&](auto with_care) __attribute__((always_inline)) {
+    auto pass = [&](auto with_care, auto from, auto to) __attribute__((always_inline)) {            // column tiles from .. to - 1
       constexpr bool careful = decltype(with_care)::value;
-      seen = 0;
+      constexpr int first = decltype(from)::value, last = decltype(to)::value;
+      constexpr uint32_t every = (1u << (2 * last)) - (1u << (2 * first));
+      seen &= ~every;
       bool ready = false;                    // all columns have one
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = first; nt < last; ++nt) {
         m[nt][0] = m[nt][1] = 0.f;
         l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
             if (2 * t + 1 < NG) y = minima[(2 * t + 1) * 8 + g];
             const uint32_t a0 = __byte_perm(x, y, 0x5410), a1 = __byte_perm(x, y, 0x7632);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = first; nt < last; ++nt) {
               const uint2 qs = qsum[nt * 32 + lane];
               mma_first(s[kb][nt], a0, a1, a0, a1, qs.x, qs.y);
               if (!kSplit)
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
                 a[kb][3] = numbers<kSplit>(x >> 8, 0x00f000f0u);
               }
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
+              for (int nt = first; nt < last; ++nt) {
                 if (kSplit) {
                   const uint4 q = *reinterpret_cast<const uint4*>(qfrag + (((2 * gr + tile) * NT + nt) * 32 + lane) * 4);
 #pragma unroll
@@ -621,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
             for (int kb = 0; kb < BK; ++kb) {
               const float2 sc = __half22float2(as_half2(reinterpret_cast<const uint32_t*>(stage + kb * 640 * NG + 512 * NG)[gr * 8 + g]));
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
+              for (int nt = first; nt < last; ++nt) {
                 s[kb][nt][0] = fmaf(sc.x, acc[kb][nt][0], s[kb][nt][0]);
                 s[kb][nt][1] = fmaf(sc.x, acc[kb][nt][1], s[kb][nt][1]);
                 s[kb][nt][2] = fmaf(sc.y, acc[kb][nt][2], s[kb][nt][2]);
@@ -633,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
           // blocks need no exchange between lanes.
           bool raise = false;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = first; nt < last; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               float top = -CUDART_INF_F;
@@ -653,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
               for (int kb = 0; kb < BK; ++kb) {
                 const bool there = bits >> kb & 1;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int nt = first; nt < last; ++nt)
 #pragma unroll
                   for (int k = 0; k < 4; ++k) {
                     const int key = key0 + kb * 16 + g + (k >= 2 ? 8 : 0), c = nt * 8 + 2 * t + (k & 1);
@@ -676,18 +678,18 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
             }
             __syncwarp();
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = first; nt < last; ++nt)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 float x = fmaxf(fmaxf(s[0][nt][k], s[0][nt][k + 2]), fmaxf(s[1][nt][k], s[1][nt][k + 2]));
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
                 const float rise = x - (careful ? kPMost : kPScale);
-                const bool first = !(seen >> (2 * nt + k) & 1);
-                if (first ? x > -CUDART_INF_F : rise > 0.f) {
+                const bool fresh = !(seen >> (2 * nt + k) & 1);
+                if (fresh ? x > -CUDART_INF_F : rise > 0.f) {
                   seen |= 1u << (2 * nt + k);
                   m[nt][k] += rise;
-                  if (!first) {
+                  if (!fresh) {
                     const float fade = exp2_fast(-rise);
                     l[nt][k] *= fade;
                     om[nt][k] *= fade;
@@ -699,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
                   for (int kb = 0; kb < BK; ++kb) { s[kb][nt][k] -= rise; s[kb][nt][k + 2] -= rise; }
                 }
               }
-            ready = __all_sync(0xffffffffu, seen == (1u << (2 * NT)) - 1u);
+            ready = __all_sync(0xffffffffu, (seen & every) == every);
           }
           // weights as halves (float32: two of them), from accumulators to B operands; then values, whose minima are an operand with groups as rows
 #pragma unroll
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
             uint2 mn = make_uint2(0, 0);
             if (g < NG) mn = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 608 * NG + g * 32 + t * 8);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = first; nt < last; ++nt) {
               float e[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) e[k] = exp2_fast(s[kb][nt][k]);
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
                 const uint2 sc = *reinterpret_cast<const uint2*>(stage + kb * 640 * NG + 576 * NG + gr * 32 + t * 8);
                 const uint32_t ox = __vcmpeq2(sc.x, 0x80008000u), oy = __vcmpeq2(sc.y, 0x80008000u);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {            // lane (g, t): row g's weights of keys 2t, 2t + 1, 2t + 8, 2t + 9
+                for (int nt = first; nt < last; ++nt) {            // lane (g, t): row g's weights of keys 2t, 2t + 1, 2t + 8, 2t + 9
                   const unsigned hit = __ballot_sync(0xffffffffu, (pb[nt][0] & ox) | (pb[nt][1] & oy));
 #pragma unroll
                   for (int k = 0; k < 2; ++k)
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
               uint32_t wb[NT][kSplit ? 4 : 2];
               if (careful) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {            // lane (g, t): row g's weights of keys 2t, 2t + 1, 2t + 8, 2t + 9
+                for (int nt = first; nt < last; ++nt) {            // lane (g, t): row g's weights of keys 2t, 2t + 1, 2t + 8, 2t + 9
                   float x[4], top = 0.f;
 #pragma unroll
                   for (int i = 0; i < 2; ++i) {
@@ -790,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
                 continue;
               }
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
+              for (int nt = first; nt < last; ++nt) {
                 if (kSplit) {
                   const float2 sx = __half22float2(as_half2(vs.x)), sy = __half22float2(as_half2(vs.y));
 #pragma unroll
@@ -812,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
                 const uint32_t a0 = numbers<kSplit>(x, 0x000f000fu), a1 = numbers<kSplit>(x, 0x00f000f0u), a2 = numbers<kSplit>(x >> 8, 0x000f000fu),
                                a3 = numbers<kSplit>(x >> 8, 0x00f000f0u);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int nt = first; nt < last; ++nt) {
                   if (kSplit) mma_split<false>(o[2 * gr + tile][nt], a0, a1, a2, a3, wb[nt][0], wb[nt][1], wb[nt][kSplit ? 2 : 0], wb[nt][kSplit ? 3 : 0]);
                   else mma_half(o[2 * gr + tile][nt], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
                 }
@@ -825,47 +827,49 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
         slot = slot + 1 == kStages ? 0 : slot + 1;
       }
     };
-    pass(std::false_type());
-    float all = 0.f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int i = 0; i < 2 * NG; ++i) all = fmaf(o[i][nt][k], 0.f, all);
-      }
-    bool again = all != 0.f;                 // NaN is not 0 either
+    pass(std::false_type(), std::integral_constant<int, 0>(), std::integral_constant<int, NT>());
+    bool again;
     {
-      // A product is off by 2^-26 (2^-25 at most) where it is subnormal, so a sum over k keys of n about 7 by sqrt(k) 2^-23: less than 2^-20 (bf16: 2^-13) of what is not smaller than this.
-      // First each lane's largest sum of four features, then the group's.  (0 is no rounding's work: the key of the largest weight has at least 2^7 2^-24.)
-      const float least = sqrtf(32.f * n_stages) * (kSplit ? 2.f : 0x1p-30f);            // in units of the high numbers, which count 16 times
+      // As bits sums ascend, 0 up to infinity and NaN.  A product is off by 2^-26 (2^-25 at most) where it is subnormal, so a sum over k keys of n about 7 by sqrt(k) 2^-23: less than 2^-18
+      // (bf16: 2^-13) of a group's largest where that is not below `least`, in units of the high numbers, which count 16 times.  (0 is no rounding's work: the key of the largest
+      // weight has at least 2^7 2^-24.)  First each lane's largest sum of four features, then the group's.
+      const uint32_t least = __float_as_uint(sqrtf(32.f * n_stages) * (kSplit ? 0.5f : 0x1p-30f)) - 1u;
       auto largest = [&](int gr, int nt, int k) __attribute__((always_inline)) {
-        return fmaxf(16.f * fmaxf(o[2 * gr][nt][k], o[2 * gr + 1][nt][k]), fmaxf(o[2 * gr][nt][k + 2], o[2 * gr + 1][nt][k + 2]));
+        return max(max(__float_as_uint(o[2 * gr][nt][k]), __float_as_uint(o[2 * gr + 1][nt][k])), max(__float_as_uint(o[2 * gr][nt][k + 2]), __float_as_uint(o[2 * gr + 1][nt][k + 2])));
       };
-      bool small = false;
+      uint32_t top = 0, lowest = 0xffffffffu;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int gr = 0; gr < NG; ++gr) small |= (seen >> (2 * nt + k) & 1) && largest(gr, nt, k) < least;
-      if (__any_sync(0xffffffffu, small)) {
+          for (int gr = 0; gr < NG; ++gr) {
+            const uint32_t x = largest(gr, nt, k);
+            top = max(top, x);
+            lowest = min(lowest, x - 1u);    // 0 is no small one
+          }
+      again = top >= 0x7f800000u;
+      if (__builtin_expect(__any_sync(0xffffffffu, lowest < least), 0)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-              float x = largest(gr, nt, k);
+              uint32_t x = largest(gr, nt, k);
 #pragma unroll
-              for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-              again |= x > 0.f && x < least;
+              for (int off = 4; off < 32; off <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, off));
+              again |= x - 1u < least;
             }
       }
     }
-    if (__any_sync(0xffffffffu, again)) {
+    if (__builtin_expect(__any_sync(0xffffffffu, again), 0)) {
       start(sg, page_at(sg, 0), page_at(sg, 1));
-      pass(std::true_type());
+      pass(std::true_type(), std::integral_constant<int, 0>(), std::integral_constant<int, 1>());
+      if constexpr (NT == 2) {               // a tile at a time, so that this takes no more registers than the quick way
+        start(sg, page_at(sg, 0), page_at(sg, 1));
+        pass(std::true_type(), std::integral_constant<int, NT - 1>(), std::integral_constant<int, NT>());
+      }
     }
 
     // ---- the next segment's keys are asked for while this one's sums become one -------------------------------------------------
