@@ -13,9 +13,10 @@
 // is shared by many CTAs.  Little work is cut into pieces of triples instead, one per CTA, if none becomes much longer than a share: a second triple costs a CTA about 7 us.  Each of a CTA's four warps takes 32 keys of a unit through a ring of bulk copies of its own, which is filled with the next triple's keys while the present
 // one's sums are joined.  Where a triple is cut, its shares leave partial sums and the last one to finish joins them (many: in groups first).
 //
-// What bounds it, in bf16 with 8 kv heads of 128 and 4 query heads each.  32 sequences of 8184 keys: 70.6 us, 4.8 TB/s, 0.73 of the copy rate; about 300 warp instructions per 16 keys and head,
-// issued at 56 % by 3.3 warps a scheduler that wait for their own arithmetic.  One sequence: 9.6 us for 300 keys, 16 for 8192, 44 for 131072; about 8 of them are the chain of lengths, table, queries, first copy and join.  float32 has three
-// products for one: 32 sequences of 4096 keys 73 us against 42.
+// What bounds it, in bf16 with 8 kv heads of 128 and 4 query heads each.  32 sequences of 8184 keys: 75 to 77 us with other inputs every call, 4.4 TB/s, 0.67 of the copy rate (70.6 over and over on the
+// same ones, of which L2 keeps a part); about 300 warp instructions per 16 keys and head, issued at 57 % by 3.3 warps a scheduler that wait for their own arithmetic.  One sequence: 9.6 us for 300 keys,
+// 16 for 8192, 44 for 131072; about 8 of them are the chain of lengths, table, queries, first copy and join.  float32 has three products for one: 32 sequences of 4096 keys 74 us against 42.  Values
+// whose products with the weights leave the halves (scales above 2^8 or so, or below 2^-14) are gone through twice: 32 x 8184 153 us recorded against 70.6, float32 32 x 4096 147 against 74.
 #pragma once
 #include <math_constants.h>
 
@@ -703,7 +704,8 @@ __global__ void __launch_bounds__(kThreads, NG >= 5 ? 2 : NT == 1 ? 4 : 3) atten
               }
             ready = __all_sync(0xffffffffu, (seen & every) == every);
           }
-          // weights as halves (float32: two of them), from accumulators to B operands; then values, whose minima are an operand with groups as rows
+          // weights as halves (float32: two of them), from accumulators to B operands; then values, whose minima are an operand with groups as rows.  bf16 rounds twice, p and p s, each by 2^-12
+          // of a term at most: beside results of unrounded weights, both rounded to bf16, 1.1e-3 of their size, where that rounding alone is 1.7e-3; a second half each would double the products
 #pragma unroll
           for (int kb = 0; kb < BK; ++kb) {
             uint32_t pb[NT][kSplit ? 4 : 2];
