@@ -605,7 +605,8 @@ int32_t lmb200_decode_attention_noalloc(lmb200_ctx ctx, int32_t dtype, const voi
  *
  * A slot or a table entry outside the cache, lengths beyond the tables and row offsets that do not ascend within the rows touch no memory: such entries and
  * sequences are left out (kv_reserve: a token whose page is such an entry, of the table or the free list, has slot -1; kv4_attention: their rows stay as they are; of offsets that
- * descend or leave the rows, all sequences are left out), and the next synchronising call returns LMB200_EINVAL.
+ * descend or leave the rows, all sequences are left out; verify_drafts: rows that such offsets give to two sequences hold tokens of either or -1), and the next synchronising call
+ * returns LMB200_EINVAL.
  * max_pages * page_size is at most 2^30.
  * ------------------------------------------------------------------------------------------ */
 int32_t lmb200_kv4_page_bytes(int32_t page_size, int32_t n_kv_heads, int32_t head_dim, int64_t* bytes);

@@ -363,7 +363,7 @@ __device__ __forceinline__ Choice decide(const VerifyParams& p, int b, int r0, i
     int token = -1;
     if (greedy) {
       const int at = best_of(stop, c.top);
-      if (c.top > -CUDART_INF_F) token = at;
+      if (c.top > -CUDART_INF_F && (unsigned)at < (unsigned)p.vocab) token = at;       // (rows that offsets give to two sequences may have no statistics)
       c.row = -1;
     } else {
       double s, sd;

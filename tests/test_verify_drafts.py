@@ -42,6 +42,38 @@ def test_verify_logits_one_step_apart_at_temperatures_near_0(on_torch, vocab, dr
     assert (want[0] >= 0).sum() >= n and (want[1] == np.where(np.arange(n) % 2 == 0, 2, 1)).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [50, 50000])
+@pytest.mark.parametrize("temperature", [None, 0.0, 1.0])
+@pytest.mark.parametrize("cu", [[0, 4, 2, 1], [0, 6, 3, 6], [2, 6, 0, 5], [0, 5, 9, 6]])
+def test_verify_offsets_that_share_rows_give_tokens_of_the_vocabulary(on_torch, vocab, temperature, cu):
+    """Whatever the workspace held: a row that offsets give to two sequences holds a token or -1, the call is told of, and the next one is right."""
+    import torch
+    L, dev = on_torch
+    rows, n = 6, 3
+    rng = np.random.default_rng(42)
+    target = cuda(rng.standard_normal((rows, vocab)).astype(np.float32))
+    tokens = rng.integers(0, vocab, rows).astype(np.int32)
+    tokens[1:] = target.argmax(1).cpu().numpy()[:-1]                        # every draft is the largest logit
+    t = None if temperature is None else torch.full((n,), temperature, device="cuda")
+    u = cuda(rng.random(rows).astype(np.float32))
+    ints = lambda k: torch.full((k,), -1, dtype=torch.int32, device="cuda")  # noqa: E731
+    for fill in (0x7f, 0x3f, 0xff):
+        ws = torch.full((L.verify_drafts_workspace(rows),), fill, dtype=torch.uint8, device="cuda")
+        out, n_out, drop = ints(rows), ints(n), ints(n)
+        L.verify_drafts(dev, target, None, cuda(np.array(cu, np.int32)), cuda(tokens), t, u, u, out, n_out, drop, workspace=ws)
+        with pytest.raises(L.LuminalB200Error) as e:
+            dev.sync()
+        assert e.value.code == -1
+        assert ((out >= -1) & (out < vocab)).all() and ((n_out >= 0) & (n_out <= rows)).all() and ((drop >= 0) & (drop < rows)).all()
+        good = np.array([0, 2, 2, 6], np.int32)
+        want = P.verify(target.cpu().numpy(), None, good, tokens, None if t is None else t.cpu().numpy(), u.cpu().numpy(), u.cpu().numpy(), np.full(rows, 55, np.int32))
+        L.verify_drafts(dev, target, None, cuda(good), cuda(tokens), t, u, u, out, n_out, drop, workspace=ws)
+        dev.sync()
+        for got, w in zip((out, n_out, drop), want):
+            assert np.array_equal(got.cpu().numpy(), w)
+
+
 # Logits below a top one at many temperatures: this exponential, CUDA's, and how far apart they may be.
 EXP64 = r"""
 #include <cmath>
